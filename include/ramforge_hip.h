@@ -20,10 +20,11 @@
  *     does; the weight bytes are the raw GGUF payload, row-major [out][in]).
  *   - `stream` is a hipStream_t; NULL selects the context's compute stream.
  *     Compute calls are asynchronous with respect to the host.
- *   - Workspaces: rf_attention_decode, rf_matmul_packed and rf_matvec_packed
- *     with a misaligned x use context-owned workspaces.  rf_ctx_reserve sizes
- *     them up front (rf_attention_workspace_bytes / rf_matmul_workspace_bytes
- *     give the bytes a shape needs) and, with fixed = 1, turns any later call
+ *   - Workspaces: rf_attention_decode, rf_attention_tree, rf_matmul_packed and
+ *     rf_matvec_packed with a misaligned x use context-owned workspaces.
+ *     rf_ctx_reserve sizes them up front (rf_attention_workspace_bytes,
+ *     rf_attention_tree_workspace_bytes and rf_matmul_workspace_bytes give the
+ *     bytes a shape needs) and, with fixed = 1, turns any later call
  *     that would need more into an RF_ERR_INVALID error: then no entry point
  *     allocates or synchronises on the hot path.  Without a fixed reservation
  *     the first call that needs a workspace (or a larger one) allocates it,
@@ -268,6 +269,105 @@ int32_t rf_attention_decode(rf_ctx *ctx, const float *q, const float *k_hist, co
 int32_t rf_attention_decode_noalloc(rf_ctx *ctx, const float *q, const float *k_hist, const float *v_hist,
                                     const float *k_cur, const float *v_cur, uint32_t hist_len, uint32_t q_heads,
                                     uint32_t kv_heads, uint32_t head_dim, float *out, rf_stream_t stream);
+
+/* ------------------------------------- drafted tokens and their cache */
+
+/* What a decode step of several tokens needs (a draft and its verification,
+ * a short prompt), with the K/V cache in few bits.  No counterparts in the
+ * reference, which decodes one token at a time over an f32 cache.  Serving
+ * only: there are no backward passes.
+ *
+ * A layer's cache: K and V buffers of rf_kv_cache_bytes each, of `capacity`
+ * positions x kv_heads x head_dim values.
+ *   RF_TYPE_F32, RF_TYPE_F16: the values, [position][kv_head][dim].
+ *   RF_TYPE_Q8_0, RF_TYPE_Q4_0: codes [position][kv_head][dim] (a byte, code +
+ *     128; half a byte, code + 8, the even dim low), then one f16 scale per 32
+ *     values [position][kv_head][dim / 32]; value = code * scale.  head_dim is
+ *     a multiple of 32.  The scale is the least f16 of at most 3 (Q8_0) or 8
+ *     (Q4_0) significant bits with 127 d >= max |x| (8 |d| >= max |x|, its
+ *     sign such that the extreme value's code is -8), so that every value is
+ *     an f16 exactly; codes are the nearest to x / d, ties to even, in
+ *     -127..127 (-8..7).  Larger magnitudes than 65024 (65280) are cut there;
+ *     a block of 32 that holds an infinity or NaN reads back as NaN.
+ *     Not the GGUF block layout.
+ * head_dim is at most 512; the buffers are 16-byte aligned.  `length`, if not
+ * NULL, is a device word that every call adds to the positions it is given
+ * (first, hist_len, src), read when the call runs: a captured graph then
+ * follows a cache that grows.  The sum is checked on the device: rows past
+ * the capacity are neither written, read nor seen (rf_kv_load leaves their
+ * outputs as they are). */
+typedef struct {
+    uint32_t type; /* RF_TYPE_F32, RF_TYPE_F16, RF_TYPE_Q8_0 or RF_TYPE_Q4_0 */
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t reserved; /* 0 */
+    uint64_t capacity;
+    void *k;
+    void *v;
+    const uint32_t *length;
+} rf_kv_cache;
+/* Bytes of each of a cache's two buffers; 0 for a type or shape not covered. */
+uint64_t rf_kv_cache_bytes(uint32_t type, uint64_t capacity, uint32_t kv_heads, uint32_t head_dim);
+/* n rows of k and v, [kv_heads][head_dim] f32 each, into positions first ..
+ * first + n - 1; and back.  Strides are in floats from one row to the next
+ * (0: rows without gaps), here and in the calls below. */
+int32_t rf_kv_store(rf_ctx *ctx, const rf_kv_cache *cache, const float *k, uint64_t k_stride, const float *v,
+                    uint64_t v_stride, uint64_t first, uint64_t n, rf_stream_t stream);
+int32_t rf_kv_load(rf_ctx *ctx, const rf_kv_cache *cache, uint64_t first, uint64_t n, float *k, uint64_t k_stride,
+                   float *v, uint64_t v_stride, rf_stream_t stream);
+/* Rows first + j take what rows src[j] (device memory) held when the call
+ * began, j < n, in every one of n_caches caches (a model's layers: one type,
+ * shape, capacity and length word; no two the same buffer): the accepted path
+ * of a draft moves to the end of the history.  n is at most 1024.  A row whose
+ * src lies past the capacity is left as it is. */
+int32_t rf_kv_move(rf_ctx *ctx, const rf_kv_cache *caches, uint32_t n_caches, const uint32_t *src, uint64_t first,
+                   uint64_t n, rf_stream_t stream);
+/* Per head of n_tokens rows of q [q_heads][head_dim] and k [kv_heads]
+ * [head_dim]: RMS norm with the weights q_norm / k_norm [head_dim] (NULL: no
+ * norm), then the half-split rotation of rf_rope by the angle positions[t] *
+ * theta^(-2 i / head_dim).  positions is device memory.  Unlike rf_rope, whose
+ * angles are the reference's f32 products, angles are computed in 64 bits;
+ * the two differ by up to position * 2^-24 radians.  An output may be its
+ * input (same address and stride), and must not overlap one otherwise.  The
+ * _store form writes the rotated k and the rows v into cache positions first
+ * .. first + n_tokens - 1 in the same pass (as rf_kv_store would); positions
+ * NULL there means the cache positions themselves.  rf_qk_norm_rope alone is
+ * also the batched rotation of a model without these norms. */
+int32_t rf_qk_norm_rope(rf_ctx *ctx, const float *q, uint64_t q_stride, const float *k, uint64_t k_stride,
+                        const float *q_norm, const float *k_norm, float eps, const uint32_t *positions,
+                        uint64_t n_tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, float theta,
+                        float *q_out, uint64_t q_out_stride, float *k_out, uint64_t k_out_stride, rf_stream_t stream);
+int32_t rf_qk_norm_rope_store(rf_ctx *ctx, const float *q, uint64_t q_stride, const float *k, uint64_t k_stride,
+                              const float *v, uint64_t v_stride, const float *q_norm, const float *k_norm, float eps,
+                              const uint32_t *positions, uint64_t n_tokens, uint32_t q_heads, float theta,
+                              float *q_out, uint64_t q_out_stride, const rf_kv_cache *cache, uint64_t first,
+                              rf_stream_t stream);
+/* The mask of a tree of n drafted tokens (at most 1024) for rf_attention_tree,
+ * once per step for all layers.  parents[i] (device memory) is the token that
+ * i continues, an earlier one, or -1 for the history's last; any other value
+ * counts as -1.  Bit j % 64 of mask[i * ceil(n / 64) + j / 64] is set where j
+ * is i or one of its ancestors.  positions, if not NULL, gets base (+ *length,
+ * if length is not NULL) plus the token's number of ancestors: the positions
+ * of rf_qk_norm_rope. */
+int32_t rf_tree_mask(rf_ctx *ctx, const int32_t *parents, uint64_t n, uint64_t base, const uint32_t *length,
+                     uint64_t *mask, uint32_t *positions, rf_stream_t stream);
+/* Attention of n tokens (at most 1024) whose k and v are cache positions
+ * hist_len .. hist_len + n - 1: each sees positions 0 .. hist_len - 1, and of
+ * the n those whose bits its row of mask has (device memory, laid out as
+ * above; NULL: a chain, tokens 0..i; n = 1 without a mask is rf_attention_decode
+ * over such a cache).  q and out are [n][q_heads][head_dim]; scores are over
+ * sqrt(head_dim), products and sums to f32 accuracy whatever the cache holds.
+ * A token that sees nothing, or only scores of minus infinity, gets zeros.
+ * What positions hold that a token does not see cannot reach it, infinities
+ * and NaN included; an infinity or NaN that it does see makes its output NaN
+ * or infinite.  Uses the attention workspace: rf_attention_tree_workspace_bytes
+ * for every call of up to max_positions (hist_len + n; with a length word, the
+ * capacity) and n tokens. */
+uint64_t rf_attention_tree_workspace_bytes(uint64_t max_positions, uint64_t n, uint32_t type, uint32_t q_heads,
+                                           uint32_t kv_heads, uint32_t head_dim);
+int32_t rf_attention_tree(rf_ctx *ctx, const float *q, uint64_t q_stride, const rf_kv_cache *cache, uint64_t hist_len,
+                          const uint64_t *mask, uint64_t n, uint32_t q_heads, float *out, uint64_t out_stride,
+                          rf_stream_t stream);
 
 /* ---------------------------------------------------------- elementwise */
 

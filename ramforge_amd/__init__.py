@@ -34,7 +34,8 @@ __all__ = [
     "GGML", "BLOCK_GEOMETRY", "Context", "DeviceArray", "RamforgeError", "ModelConfig",
     "matvec", "dequantize_rows", "attention_checked", "apply_rope", "rmsnorm", "add", "mul",
     "silu", "swiglu", "softmax", "argmax", "GpuBackend", "GpuTensor", "matvec_backend",
-    "GpuLlamaModel", "row_bytes",
+    "GpuLlamaModel", "row_bytes", "KvCache", "KvCacheList", "kv_cache_bytes", "kv_store", "kv_load", "kv_move", "qk_norm_rope",
+    "qk_norm_rope_store", "tree_mask", "attention_tree",
 ]
 
 
@@ -188,6 +189,11 @@ class Context:
 
     def attention_workspace_bytes(self, max_positions: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
         return int(self.lib.rf_attention_workspace_bytes(max_positions, n_heads, n_kv_heads, head_dim))
+
+    def attention_tree_workspace_bytes(self, max_positions: int, n: int, ggml_type: int, n_heads: int,
+                                       n_kv_heads: int, head_dim: int) -> int:
+        return int(self.lib.rf_attention_tree_workspace_bytes(max_positions, n, ggml_type, n_heads, n_kv_heads,
+                                                              head_dim))
 
     def matmul_workspace_bytes(self, out_dim: int, in_dim: int, n_tokens: int) -> int:
         return int(self.lib.rf_matmul_workspace_bytes(out_dim, in_dim, n_tokens))
@@ -470,6 +476,133 @@ def argmax(ctx: Context, logits, n: int, out_index, stream=None) -> None:
     """Greedy Sampler::sample_checked (sampling.rs:45-57) into device memory."""
     _fits("argmax", logits=(logits, 4 * n), out_index=(out_index, 4))
     _lib.check(ctx.lib.rf_argmax(ctx.handle, _ptr(logits), n, _ptr(out_index), stream))
+
+
+# ------------------------------------------------ drafted tokens, their cache
+
+class KvCache:
+    """A layer's K/V cache of ``capacity`` positions in F32, F16, Q8_0 or Q4_0 (rf_kv_cache).  ``k`` and ``v`` are
+    device buffers of kv_cache_bytes() each (allocated here if not given), ``length`` a device uint32 that every
+    call adds to the positions it is given, or None."""
+
+    def __init__(self, ctx: Context, ggml_type: int, capacity: int, n_kv_heads: int, head_dim: int, k=None, v=None,
+                 length=None):
+        nbytes = kv_cache_bytes(ggml_type, capacity, n_kv_heads, head_dim)
+        self.owned = []
+        if nbytes and (k is None or v is None):
+            k = ctx.alloc(nbytes) if k is None else k
+            v = ctx.alloc(nbytes) if v is None else v
+            self.owned = [b for b in (k, v) if isinstance(b, DeviceArray)]
+        if nbytes:
+            _fits("KV cache", k=(k, nbytes), v=(v, nbytes))
+        self.ctx, self.type, self.capacity, self.n_kv_heads, self.head_dim = ctx, ggml_type, capacity, n_kv_heads, head_dim
+        self.k, self.v, self.length = k, v, length
+        self.struct = _lib.KvCacheStruct(ggml_type, n_kv_heads, head_dim, 0, capacity, _ptr(k), _ptr(v), _ptr(length))
+        self.ref = C.addressof(self.struct)
+
+    @property
+    def width(self) -> int:
+        return self.n_kv_heads * self.head_dim
+
+    def free(self) -> None:
+        """Frees the buffers this object allocated."""
+        for b in self.owned:
+            b.free()
+        self.owned = []
+
+
+class KvCacheList:
+    """The caches of a model's layers, for kv_move."""
+
+    def __init__(self, caches: Sequence[KvCache]):
+        self.caches = list(caches)
+        self.array = (_lib.KvCacheStruct * max(len(self.caches), 1))(*(c.struct for c in self.caches))
+        self.ref, self.n = C.addressof(self.array), len(self.caches)
+
+
+def kv_cache_bytes(ggml_type: int, capacity: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of each of a cache's two buffers (0: a type or shape the cache does not cover)."""
+    return int(_lib.load().rf_kv_cache_bytes(ggml_type, capacity, n_kv_heads, head_dim))
+
+
+def _span(n: int, width: int, stride: int) -> int:
+    """Bytes that n rows of width floats, stride apart, reach over."""
+    return 4 * ((n - 1) * (stride or width) + width) if n else 0
+
+
+def kv_store(ctx: Context, cache: KvCache, k, v, first: int, n: int, k_stride: int = 0, v_stride: int = 0,
+             stream=None) -> None:
+    """n rows of k and v ([n_kv_heads][head_dim] f32, strides in floats) into cache positions first .. first + n - 1."""
+    _fits("KV store", k=(k, _span(n, cache.width, k_stride)), v=(v, _span(n, cache.width, v_stride)))
+    _lib.check(ctx.lib.rf_kv_store(ctx.handle, cache.ref, _ptr(k), k_stride, _ptr(v), v_stride, first, n, stream))
+
+
+def kv_load(ctx: Context, cache: KvCache, first: int, n: int, k, v, k_stride: int = 0, v_stride: int = 0,
+            stream=None) -> None:
+    """Cache positions first .. first + n - 1 as rows of k and v (f32)."""
+    _fits("KV load", k=(k, _span(n, cache.width, k_stride)), v=(v, _span(n, cache.width, v_stride)))
+    _lib.check(ctx.lib.rf_kv_load(ctx.handle, cache.ref, first, n, _ptr(k), k_stride, _ptr(v), v_stride, stream))
+
+
+def kv_move(ctx: Context, caches, src, first: int, n: int, stream=None) -> None:
+    """In each cache (a KvCacheList, or a sequence of KvCache) positions first + j take what positions src[j] (device
+    uint32) held before: an accepted path of drafts moves to the end of the history."""
+    if not isinstance(caches, KvCacheList):
+        caches = KvCacheList(caches)
+    _fits("KV move", src=(src, 4 * n))
+    _lib.check(ctx.lib.rf_kv_move(ctx.handle, caches.ref, caches.n, _ptr(src), first, n, stream))
+
+
+def qk_norm_rope(ctx: Context, q, k, q_norm, k_norm, eps: float, positions, n_tokens: int, n_heads: int,
+                 n_kv_heads: int, head_dim: int, freq_base: float, q_out, k_out, q_stride: int = 0, k_stride: int = 0,
+                 q_out_stride: int = 0, k_out_stride: int = 0, stream=None) -> None:
+    """RMS norm of every query and key head (weights None: no norm) and half-split RoPE at positions[t] (device
+    uint32), n_tokens rows in one pass."""
+    qd, kvd = n_heads * head_dim, n_kv_heads * head_dim
+    _fits("QK norm and RoPE", q=(q, _span(n_tokens, qd, q_stride)), k=(k, _span(n_tokens, kvd, k_stride)),
+          q_norm=(q_norm, 4 * head_dim), k_norm=(k_norm, 4 * head_dim), positions=(positions, 4 * n_tokens),
+          q_out=(q_out, _span(n_tokens, qd, q_out_stride)), k_out=(k_out, _span(n_tokens, kvd, k_out_stride)))
+    _lib.check(ctx.lib.rf_qk_norm_rope(ctx.handle, _ptr(q), q_stride, _ptr(k), k_stride, _ptr(q_norm), _ptr(k_norm),
+                                       eps, _ptr(positions), n_tokens, n_heads, n_kv_heads, head_dim, freq_base,
+                                       _ptr(q_out), q_out_stride, _ptr(k_out), k_out_stride, stream))
+
+
+def qk_norm_rope_store(ctx: Context, q, k, v, q_norm, k_norm, eps: float, positions, n_tokens: int, n_heads: int,
+                       freq_base: float, q_out, cache: KvCache, first: int, q_stride: int = 0, k_stride: int = 0,
+                       v_stride: int = 0, q_out_stride: int = 0, stream=None) -> None:
+    """qk_norm_rope with the rotated k and the rows v written into cache positions first .. in the same pass
+    (positions None: the cache positions)."""
+    qd, kvd = n_heads * cache.head_dim, cache.width
+    _fits("QK norm and RoPE store", q=(q, _span(n_tokens, qd, q_stride)), k=(k, _span(n_tokens, kvd, k_stride)),
+          v=(v, _span(n_tokens, kvd, v_stride)), q_norm=(q_norm, 4 * cache.head_dim),
+          k_norm=(k_norm, 4 * cache.head_dim), positions=(positions, 4 * n_tokens),
+          q_out=(q_out, _span(n_tokens, qd, q_out_stride)))
+    _lib.check(ctx.lib.rf_qk_norm_rope_store(ctx.handle, _ptr(q), q_stride, _ptr(k), k_stride, _ptr(v), v_stride,
+                                             _ptr(q_norm), _ptr(k_norm), eps, _ptr(positions), n_tokens, n_heads,
+                                             freq_base, _ptr(q_out), q_out_stride, cache.ref, first, stream))
+
+
+def tree_mask(ctx: Context, parents, n: int, base: int, mask, positions=None, length=None, stream=None) -> None:
+    """The ancestor mask ([n][ceil(n / 64)] uint64) of a tree of n drafted tokens from their parents (device int32,
+    -1: the history), and their positions, base plus depth (uint32)."""
+    _fits("tree mask", parents=(parents, 4 * n), mask=(mask, 8 * n * ((n + 63) // 64)), positions=(positions, 4 * n))
+    _lib.check(ctx.lib.rf_tree_mask(ctx.handle, _ptr(parents), n, base, _ptr(length), _ptr(mask), _ptr(positions),
+                                    stream))
+
+
+def attention_tree(ctx: Context, q, cache: KvCache, hist_len: int, n: int, n_heads: int, mask=None,
+                   out: Optional[DeviceArray] = None, q_stride: int = 0, out_stride: int = 0,
+                   stream=None) -> DeviceArray:
+    """Attention of n tokens at cache positions hist_len .. hist_len + n - 1, over the history and what their mask
+    rows allow of one another (mask None: a chain)."""
+    qd = n_heads * cache.head_dim
+    _fits("tree attention", q=(q, _span(n, qd, q_stride)), out=(out, _span(n, qd, out_stride)),
+          mask=(mask, 8 * n * ((n + 63) // 64)))
+    if out is None:
+        out = ctx.empty((n, qd) if out_stride in (0, qd) else (n, out_stride))
+    _lib.check(ctx.lib.rf_attention_tree(ctx.handle, _ptr(q), q_stride, cache.ref, hist_len, _ptr(mask), n, n_heads,
+                                         _ptr(out), out_stride, stream))
+    return out
 
 
 # ------------------------------------------------- backend / dispatch mirror

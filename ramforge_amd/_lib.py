@@ -54,6 +54,21 @@ class ModelConfig(C.Structure):
     ]
 
 
+class KvCacheStruct(C.Structure):
+    """rf_kv_cache: a layer's K and V buffers."""
+
+    _fields_ = [
+        ("type", _u32),
+        ("kv_heads", _u32),
+        ("head_dim", _u32),
+        ("reserved", _u32),
+        ("capacity", _u64),
+        ("k", _vp),
+        ("v", _vp),
+        ("length", _vp),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "rf_last_error": (C.c_size_t, [C.c_char_p, C.c_size_t]),
@@ -98,6 +113,17 @@ SIGNATURES = {
     "rf_dequantize_rows": (_i32, [_vp, _u32, _vp, _u64, _u64, _u64, _u64, _fp, _vp]),
     "rf_attention_decode": (_i32, [_vp, _fp, _fp, _fp, _fp, _fp, _u32, _u32, _u32, _u32, _fp, _vp]),
     "rf_attention_decode_noalloc": (_i32, [_vp, _fp, _fp, _fp, _fp, _fp, _u32, _u32, _u32, _u32, _fp, _vp]),
+    "rf_kv_cache_bytes": (_u64, [_u32, _u64, _u32, _u32]),
+    "rf_kv_store": (_i32, [_vp, _vp, _fp, _u64, _fp, _u64, _u64, _u64, _vp]),
+    "rf_kv_load": (_i32, [_vp, _vp, _u64, _u64, _fp, _u64, _fp, _u64, _vp]),
+    "rf_kv_move": (_i32, [_vp, _vp, _u32, _vp, _u64, _u64, _vp]),
+    "rf_qk_norm_rope": (_i32, [_vp, _fp, _u64, _fp, _u64, _fp, _fp, _f32, _vp, _u64, _u32, _u32, _u32, _f32, _fp,
+                               _u64, _fp, _u64, _vp]),
+    "rf_qk_norm_rope_store": (_i32, [_vp, _fp, _u64, _fp, _u64, _fp, _u64, _fp, _fp, _f32, _vp, _u64, _u32, _f32,
+                                     _fp, _u64, _vp, _u64, _vp]),
+    "rf_tree_mask": (_i32, [_vp, _vp, _u64, _u64, _vp, _vp, _vp, _vp]),
+    "rf_attention_tree_workspace_bytes": (_u64, [_u64, _u64, _u32, _u32, _u32, _u32]),
+    "rf_attention_tree": (_i32, [_vp, _fp, _u64, _vp, _u64, _vp, _u64, _u32, _fp, _u64, _vp]),
     "rf_rope": (_i32, [_vp, _fp, _fp, _u64, _u32, _u32, _u32, _f32, _vp]),
     "rf_rmsnorm": (_i32, [_vp, _fp, _fp, _u64, _f32, _fp, _vp]),
     "rf_add": (_i32, [_vp, _fp, _fp, _u64, _fp, _vp]),

@@ -1,6 +1,7 @@
 // rf_runtime.hip — context, device-memory ledger and the op entry points of
 // the C ABI (include/ramforge_hip.h).  Host code; kernels live in the other
 // translation units.
+#include "rf_kv.h"
 #include "rf_runtime.h"
 
 #include <algorithm>
@@ -383,7 +384,7 @@ int32_t rf_ctx_create(int32_t device, uint64_t budget, rf_ctx** out) {
   // stream capture (rf_model_decode_steps, rf_capture_begin), where the
   // load's own device allocation and copies are not capturable work.
   for (hipError_t (*load)() : {load_module_attention, load_module_elementwise, load_module_matvec,
-                               load_module_packed, load_module_prefill}) {
+                               load_module_packed, load_module_prefill, load_module_kv, load_module_tree}) {
     e = load();
     if (e != hipSuccess) {
       rc = hip_error(e, "loading the kernel code objects");
