@@ -243,6 +243,7 @@ int32_t rf_attention_tree(rf_ctx* ctx, const float* q, uint64_t q_stride, const 
   if (!q || !out) return set_error(RF_ERR_INVALID, "tree attention received a null pointer");
   a.q = q; a.q_stride = q_stride; a.out = out; a.out_stride = out_stride; a.mask = mask;
   a.hist = hist_len; a.n = (uint32_t)n; a.qh = q_heads;
+  a.q_vec = (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && q_stride % 4 == 0;
   // with a length word the context may grow to the whole cache under a captured call
   const uint64_t total = a.cache.length ? a.cache.cap : hist_len + n;
   a.nsplit = tree_splits(total, a.n, q_heads, a.cache.kvh, a.cache.hd, a.cache.type);

@@ -78,6 +78,7 @@ struct TreeArgs {
   uint64_t hist;
   uint32_t n, qh;
   uint32_t nsplit;  // position splits; > 1: records in ws
+  uint32_t q_vec;   // q rows are 16-byte aligned
   float* ws;
 };
 // Splits of a call over `total` positions, and the workspace floats they need.

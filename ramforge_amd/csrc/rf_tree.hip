@@ -5,6 +5,8 @@
 // a token's ancestors and itself).  out = softmax(q K^T / sqrt(hd)) V per query
 // head, query head h reading KV head h * kvh / qh.  Rows that see nothing are
 // zeros.
+#include <type_traits>
+
 #include "rf_device.h"
 #include "rf_kernels.h"
 #include "rf_kv.h"
@@ -234,8 +236,8 @@ template <uint32_t T, int HD> struct TreeTile {
   uint32_t ks[2][KS ? KS : 1], vs[8][VS ? VS : 1];
 
   // kr, vr: the tile's rows of codes; ksr, vsr: of scales.  row, srow: bytes of a position.
-  __device__ __forceinline__ void load(TreeRsrc kr, TreeRsrc ksr, TreeRsrc vr, TreeRsrc vsr, uint32_t row,
-                                       uint32_t srow, uint32_t head, uint32_t c, uint32_t g) {
+  __device__ __forceinline__ void load_k(TreeRsrc kr, TreeRsrc ksr, uint32_t row, uint32_t srow, uint32_t head,
+                                         uint32_t c, uint32_t g) {
     const uint32_t hb = head * (HD * BITS / 8), hs = head * (HD / 16);
 #pragma unroll
     for (uint32_t t = 0; t < 2; ++t) {
@@ -249,6 +251,10 @@ template <uint32_t T, int HD> struct TreeTile {
         }
       }
     }
+  }
+  __device__ __forceinline__ void load_v(TreeRsrc vr, TreeRsrc vsr, uint32_t row, uint32_t srow, uint32_t head,
+                                         uint32_t c, uint32_t g) {
+    const uint32_t hb = head * (HD * BITS / 8), hs = head * (HD / 16);
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
       const uint32_t p = 16u * (j / 4u) + 4u * g + j % 4u;
@@ -263,52 +269,66 @@ template <uint32_t T, int HD> struct TreeTile {
   // Element i of a lane's Q for step s goes with dim 8 s + order(i) of its HD / 4.
   static __device__ __forceinline__ constexpr int order(int i) { return T == T_Q4_0 ? (i / 2) + 4 * (i % 2) : i; }
 
+  // The eight halves of a step's K words.
+  static __device__ __forceinline__ void decode_k(const uint32_t* k, uint32_t scale, u32x4& w) {
+    const uint32_t s2 = scale | scale << 16;
+    if constexpr (T == T_Q8_0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w[2 * i] = pk_mul(pk_q8(__builtin_amdgcn_perm(0u, k[i], 0x0C010C00u)), s2);
+        w[2 * i + 1] = pk_mul(pk_q8(__builtin_amdgcn_perm(0u, k[i], 0x0C030C02u)), s2);
+      }
+    } else {
+      w[0] = pk_mul(pk_q4<0>(k[0]), s2);
+      w[1] = pk_mul(pk_q4<1>(k[0]), s2);
+      w[2] = pk_mul(pk_q4<2>(k[0]), s2);
+      w[3] = pk_mul(pk_q4<3>(k[0]), s2);
+    }
+  }
   __device__ __forceinline__ half8_t kfrag(int t, int s) const {
     u32x4 w;
     if constexpr (T == T_F16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = k[t][4 * s + i];
     } else {
-      const uint32_t sc = ks[t][HD == 96 ? s : s / 4], sc2 = sc | sc << 16;
-      if constexpr (T == T_Q8_0) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t x = k[t][2 * s + i];
-          w[2 * i] = pk_mul(pk_q8(__builtin_amdgcn_perm(0u, x, 0x0C010C00u)), sc2);
-          w[2 * i + 1] = pk_mul(pk_q8(__builtin_amdgcn_perm(0u, x, 0x0C030C02u)), sc2);
-        }
-      } else {
-        const uint32_t x = k[t][s];
-        w[0] = pk_mul(pk_q4<0>(x), sc2);
-        w[1] = pk_mul(pk_q4<1>(x), sc2);
-        w[2] = pk_mul(pk_q4<2>(x), sc2);
-        w[3] = pk_mul(pk_q4<3>(x), sc2);
-      }
+      decode_k(k[t] + s * (BITS / 4), ks[t][HD == 96 ? s : s / 4], w);
     }
     return __builtin_bit_cast(half8_t, w);
+  }
+  // The halves of two positions a, b at dim TILE of the lane's
+  template <int TILE>
+  static __device__ __forceinline__ uint32_t pair(const uint32_t* va, const uint32_t* vb, const uint32_t* sa, const uint32_t* sb) {
+    constexpr int seg = TILE < D::W0 ? 0 : 1, e = seg ? TILE - D::W0 : TILE, per = 32 / BITS;  // element e of the lane's dims
+    constexpr int word = (seg ? VW0 : 0) + e / per, in = e % per;
+    const uint32_t a = va[word], b = vb[word];
+    if constexpr (T == T_F16) {
+      return __builtin_amdgcn_perm(b, a, in ? 0x07060302u : 0x05040100u);
+    } else {
+      const uint32_t s2 = sa[seg] | sb[seg] << 16;
+      if constexpr (T == T_Q8_0) {
+        return pk_mul(pk_q8(__builtin_amdgcn_perm(b, a, 0x0C040C00u + 0x00010001u * in)), s2);
+      } else {
+        const uint32_t x = __builtin_amdgcn_perm(b, a, in < 4 ? 0x05040100u : 0x07060302u);
+        return pk_mul(pk_q4<in % 4>(x), s2);
+      }
+    }
   }
   // V^T's tile of 16 dims
   template <int TILE>
   __device__ __forceinline__ half8_t vfrag() const {
-    constexpr int seg = TILE < D::W0 ? 0 : 1, e = seg ? TILE - D::W0 : TILE, per = 32 / BITS;  // element e of the lane's dims
-    constexpr int word = (seg ? VW0 : 0) + e / per, in = e % per;
     u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a = v[2 * i][word], b = v[2 * i + 1][word];
-      if constexpr (T == T_F16) {
-        w[i] = __builtin_amdgcn_perm(b, a, in ? 0x07060302u : 0x05040100u);
-      } else {
-        const uint32_t s2 = vs[2 * i][seg] | vs[2 * i + 1][seg] << 16;
-        if constexpr (T == T_Q8_0) {
-          w[i] = pk_mul(pk_q8(__builtin_amdgcn_perm(b, a, 0x0C040C00u + 0x00010001u * in)), s2);
-        } else {
-          const uint32_t x = __builtin_amdgcn_perm(b, a, in < 4 ? 0x05040100u : 0x07060302u);
-          w[i] = pk_mul(pk_q4<in % 4>(x), s2);
-        }
-      }
-    }
+    for (int i = 0; i < 4; ++i) w[i] = pair<TILE>(v[2 * i], v[2 * i + 1], vs[2 * i], vs[2 * i + 1]);
     return __builtin_bit_cast(half8_t, w);
+  }
+  // One word of all tiles' operands, from two positions
+  template <int TILE = 0>
+  static __device__ __forceinline__ void decode_v(const uint32_t* va, const uint32_t* vb, const uint32_t* sa,
+                                                  const uint32_t* sb, uint32_t (&w)[D::TILES]) {
+    if constexpr (TILE < D::TILES) {
+      w[TILE] = pair<TILE>(va, vb, sa, sb);
+      decode_v<TILE + 1>(va, vb, sa, sb, w);
+    }
   }
 };
 
@@ -317,10 +337,13 @@ template <int HD> struct TreeTile<T_F32, HD> {
   using D = TreeDims<HD>;
   static constexpr bool QUANT = false;
   uint32_t k[2][HD / 4], v[8][HD / 16];
-  __device__ __forceinline__ void load(TreeRsrc kr, TreeRsrc, TreeRsrc vr, TreeRsrc, uint32_t row, uint32_t,
-                                       uint32_t head, uint32_t c, uint32_t g) {
+  __device__ __forceinline__ void load_k(TreeRsrc kr, TreeRsrc, uint32_t row, uint32_t, uint32_t head, uint32_t c,
+                                         uint32_t g) {
 #pragma unroll
     for (uint32_t t = 0; t < 2; ++t) tree_words<HD / 4>(k[t], kr, (16u * t + c) * row + head * (HD * 4u) + g * HD);
+  }
+  __device__ __forceinline__ void load_v(TreeRsrc vr, TreeRsrc, uint32_t row, uint32_t, uint32_t head, uint32_t c,
+                                         uint32_t g) {
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
       const uint32_t off = (16u * (j / 4u) + 4u * g + j % 4u) * row + head * (HD * 4u);
@@ -338,370 +361,764 @@ constexpr float TREE_FLOOR = -1e30f;  // reference of a row that has seen nothin
 constexpr float TREE_BELOW = 12.f, TREE_MOST = 15.f;
 constexpr uint32_t TREE_WAVES = 4, TREE_KEYS = 32;
 
-template <uint32_t T, int HD, int M, int TILE>
-__device__ __forceinline__ void tree_tiles(const TreeTile<T, HD>& x, const half8_t (&ph)[M], const half8_t (&pl)[M],
-                                           bool drafts, bool& odd, f32x4 (&o)[M][TreeDims<HD>::TILES]) {
-  if constexpr (TILE < TreeDims<HD>::TILES) {
-    half8_t vf = x.template vfrag<TILE>();
-    if (drafts) {
-      u32x4 w = __builtin_bit_cast(u32x4, vf);
+__device__ __forceinline__ void tree_lds_order() {  // within a wavefront
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Two f16 pieces of x and y: the nearest halves, and the nearest of what they leave.
+__device__ __forceinline__ void tree_pieces(float x, float y, uint32_t& hi, uint32_t& lo) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const half2_t h = __builtin_convertvector((f32x2{x, y}), half2_t);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{fmaf((float)h[0], -1.f, x), fmaf((float)h[1], -1.f, y)}), half2_t));
+}
+
+// Shared memory of a workgroup: Q's operands (all its wavefronts have the same
+// rows), and rows of sums, where the wavefronts join and odd values are added.
+template <uint32_t T, int HD, int M> struct TreeShared {
+  static constexpr uint32_t CH = HD < 128 ? HD : 128, PARTS = HD / CH, OP = CH + 4;  // dims of a part of an output row
+  static constexpr uint32_t QW = T == T_F32 ? HD / 16 : HD / 16;  // 16-byte words of a lane's Q
+  u32x4 q[M][QW][64];
+  float scale[M][16];
+  float sum[TREE_WAVES][16 * OP];
+  float m[TREE_WAVES][M * 16], l[TREE_WAVES][M * 16];
+};
+
+// A lane's HD / 4 values of a row of q.
+template <int HD>
+__device__ __forceinline__ void tree_get_q(float (&x)[HD / 4], const float* qp, bool vec) {
+  if (vec) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t keep = ((w[i] & 0x7C00u) == 0x7C00u ? 0u : 0xFFFFu) | ((w[i] & 0x7C000000u) == 0x7C000000u ? 0u : 0xFFFF0000u);
-        odd |= keep != 0xFFFFFFFFu;
-        w[i] &= keep;
-      }
-      vf = __builtin_bit_cast(half8_t, w);
+    for (int e = 0; e < HD / 16; ++e) {
+      const float4 v = reinterpret_cast<const float4*>(qp)[e];
+      x[4 * e] = v.x; x[4 * e + 1] = v.y; x[4 * e + 2] = v.z; x[4 * e + 3] = v.w;
     }
+  } else {
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      o[m][TILE] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[m], o[m][TILE], 0, 0, 0);
-      o[m][TILE] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[m], o[m][TILE], 0, 0, 0);
-    }
-    tree_tiles<T, HD, M, TILE + 1>(x, ph, pl, drafts, odd, o);
+    for (int e = 0; e < HD / 4; ++e) x[e] = qp[e];
   }
+}
+
+// Their two pieces of every step, put(step, piece, eight halves), piece 1 the
+// first and 0 the rest, scaled to 2^10 .. 2^11 by a power of two; the scale
+// that takes the scores to powers of two is returned.
+template <uint32_t T, int HD, typename Put>
+__device__ __forceinline__ float tree_split_q(const float (&x)[HD / 4], Put put) {
+  float scale = 1.44269504088896340736f / sqrtf((float)HD), top = 0.f, up = 1.f;
+#pragma unroll
+  for (int i = 0; i < HD / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  if (top > 0x1p-100f && top <= 3.402823466e38f) {
+    const uint32_t e = __float_as_uint(top) >> 23;  // biased
+    up = __uint_as_float((264u - e) << 23);         // 2^(10 - (e - 127))
+    scale *= __uint_as_float((e - 10u) << 23);
+  }
+#pragma unroll
+  for (int s = 0; s < HD / 32; ++s) {
+    u32x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      using Tile = TreeTile<T, HD>;
+      uint32_t h, r;
+      tree_pieces(x[8 * s + Tile::order(2 * i)] * up, x[8 * s + Tile::order(2 * i + 1)] * up, h, r);
+      hi[i] = h;
+      lo[i] = r;
+    }
+    put(s, 0, lo);
+    put(s, 1, hi);
+  }
+  return scale;
+}
+
+// Q's operands of row tile m, by one wavefront.  f16 caches: word 2 s + piece of lane l is its eight halves of step s.
+// An f32 cache: word i is four floats.
+template <uint32_t T, int HD, int M>
+__device__ __forceinline__ void tree_put_q(TreeShared<T, HD, M>& sh, int m, float (&x)[HD / 4], uint32_t lane) {
+  float scale = 1.44269504088896340736f / sqrtf((float)HD);  // of the scores, to powers of two
+  if constexpr (T == T_F32) {
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(x[4 * i + e]);
+      sh.q[m][i][lane] = w;
+    }
+  } else {
+    scale = tree_split_q<T, HD>(x, [&](int s, int piece, u32x4 w) { sh.q[m][2 * s + piece][lane] = w; });
+  }
+  if (lane < 16u) sh.scale[m][lane] = scale;
 }
 
 // Non-finite values of the tile's drafted V rows must not meet the zero
 // weights of rows that do not see them: they are taken out of the operand and
 // added, by value, to the rows that do.  Rare, so plain and slow; the sums go
-// through this wavefront's LDS rows so that no register array is indexed.
-template <uint32_t T, int HD, int M>
+// through 16 x TREE_ODD floats of LDS, 32 dims at a time, so that no register
+// array is indexed.
+constexpr uint32_t TREE_ODD = 36;
+template <int HD, int M>
 __device__ __forceinline__ void tree_odd_rows(const TreeArgs& a, const float (&p)[M][8], const uint32_t (&see)[M],
                                               uint64_t p0, uint64_t total, uint32_t head, uint32_t c, uint32_t g,
                                               float* lds, f32x4 (&o)[M][TreeDims<HD>::TILES]) {
   using D = TreeDims<HD>;
   const uint32_t np = (uint32_t)min((uint64_t)TREE_KEYS, total - p0);
-  float* const mine = lds + c * (HD + 4);
+  float* const mine = lds + c * TREE_ODD;
 #pragma unroll
   for (int m = 0; m < M; ++m) {
 #pragma unroll 1
-    for (uint32_t d = g; d < (uint32_t)HD; d += 4u) mine[d] = 0.f;
+    for (uint32_t part = 0; part < (uint32_t)HD / 32u; ++part) {
 #pragma unroll 1
-    for (uint32_t k = 0; k < np; ++k) {
-      const uint32_t j = 4u * (k / 16u) + k % 4u;
-      const int from = (int)((k % 16u / 4u) * 16u + c);  // the lane that holds row c's weight of position k
-      float w = 0.f;
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) w = i == j ? p[m][i] : w;
-      w = __shfl(w, from);
-      const bool sees = (uint32_t)__shfl((int)see[m], from) >> j & 1u;
+      for (uint32_t d = g; d < 32u; d += 4u) mine[d] = 0.f;
 #pragma unroll 1
-      for (uint32_t d = g; d < (uint32_t)HD; d += 4u) {
-        const float x = kv_value(a.cache.v, a.cache, p0 + k, head * HD + d);
-        if (sees && !(fabsf(x) <= 3.402823466e38f)) mine[d] += w * x;
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+      for (uint32_t k = 0; k < np; ++k) {
+        const uint32_t j = 4u * (k / 16u) + k % 4u;
+        const int from = (int)((k % 16u / 4u) * 16u + c);  // the lane that holds row c's weight of position k
+        float w = 0.f;
 #pragma unroll
-    for (int d = 0; d < D::TILES; ++d)
-#pragma unroll
-      for (uint32_t v = 0; v < 4; ++v) o[m][d][v] += mine[D::dim(d, 4u * g + v)];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-}
-
-// O^T += V^T P^T
-template <uint32_t T, int HD, int M>
-__device__ __forceinline__ void tree_weigh(const TreeArgs& a, const TreeTile<T, HD>& x, const float (&p)[M][8],
-                                           const uint32_t (&see)[M], bool drafts, uint64_t p0, uint64_t total,
-                                           uint32_t head, uint32_t c, uint32_t g, float* lds,
-                                           f32x4 (&o)[M][TreeDims<HD>::TILES]) {
-  using D = TreeDims<HD>;
-  bool odd = false;
-  if constexpr (T == T_F32) {
-#pragma unroll
-    for (int d = 0; d < D::TILES; ++d)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float v = __uint_as_float(x.v[j][d]);
-        if (drafts && !(fabsf(v) <= 3.402823466e38f)) {
-          odd = true;
-          v = 0.f;
+        for (uint32_t i = 0; i < 8; ++i) w = i == j ? p[m][i] : w;
+        w = __shfl(w, from);
+        const bool sees = (uint32_t)__shfl((int)see[m], from) >> j & 1u;
+#pragma unroll 1
+        for (uint32_t d = g; d < 32u; d += 4u) {
+          const float x = kv_value(a.cache.v, a.cache, p0 + k, head * HD + part * 32u + d);
+          if (sees && !(fabsf(x) <= 3.402823466e38f)) mine[d] += w * x;
         }
-#pragma unroll
-        for (int m = 0; m < M; ++m) o[m][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[m][j], o[m][d], 0, 0, 0);
       }
-  } else {
-    half8_t ph[M], pl[M];
+      tree_lds_order();
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+      for (int d = 0; d < D::TILES; ++d)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ph[m][j] = (_Float16)p[m][j];
-        pl[m][j] = (_Float16)(p[m][j] - (float)ph[m][j]);
-      }
-    tree_tiles<T, HD, M, 0>(x, ph, pl, drafts, odd, o);
+        for (uint32_t v = 0; v < 4; ++v) {
+          const uint32_t dim = D::dim(d, 4u * g + v);
+          if (dim / 32u == part) o[m][d][v] += mine[dim % 32u];
+        }
+      tree_lds_order();
+    }
   }
-  if (drafts && __any(odd)) tree_odd_rows<T, HD, M>(a, p, see, p0, total, head, c, g, lds, o);
 }
 
+// What a row tile's scores do to its state: masked ones out, the reference,
+// weights, their sum.  s comes in as raw sums of products.
+template <int HD, bool DRAFTS>
+__device__ __forceinline__ void tree_soften(f32x4 (&s)[2], uint32_t see, float scale, float& ref, float& l,
+                                            f32x4 (&o)[TreeDims<HD>::TILES], float (&p)[8]) {
+  if constexpr (DRAFTS) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j / 4][j % 4] = see >> j & 1u ? s[j / 4][j % 4] : -INFINITY;
+  }
+  float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                    fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+  // The reference stays until a weight would pass 2^15: few tiles rescale.
+  if (__any(fmaf(top, scale, -ref) > TREE_MOST)) {
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float now = fmaxf(ref, fmaf(top, scale, -TREE_BELOW)), al = exp2f(ref - now);
+    ref = now;
+    l *= al;
+#pragma unroll
+    for (int d = 0; d < TreeDims<HD>::TILES; ++d)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) o[d][v] *= al;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], scale, -ref));
+  l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+}
+
+// The places of a lane (4 t + v: position p0 + 16 t + 4 g + v) that token i sees.
+__device__ __forceinline__ uint32_t tree_places(const TreeArgs& a, uint32_t words, uint32_t i, uint64_t p0,
+                                                uint64_t hist, uint64_t total, uint32_t g) {
+  const uint32_t w = tree_window(a, words, i, (int64_t)(p0 - hist), (uint32_t)(total - hist)) >> 4u * g;
+  return (w & 15u) | (w >> 12 & 0xF0u);
+}
+
+// A tile of V^T without its non-finite values.
+__device__ __forceinline__ half8_t tree_finite(half8_t v, bool& odd) {
+  u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t keep =
+        ((w[k] & 0x7C00u) == 0x7C00u ? 0u : 0xFFFFu) | ((w[k] & 0x7C000000u) == 0x7C000000u ? 0u : 0xFFFF0000u);
+    odd |= keep != 0xFFFFFFFFu;
+    w[k] &= keep;
+  }
+  return __builtin_bit_cast(half8_t, w);
+}
+
+// O^T += V^T P^T for the f16 forms, N dim tiles at a time: the first of the
+// pieces for all of them, then the other, so that no instruction waits for the
+// sum before it.  DRAFTS: non-finite values are taken out (see above).
+template <uint32_t T, int HD, int M, bool DRAFTS, int TILE>
+__device__ __forceinline__ void tree_tiles(const TreeTile<T, HD>& x, const u32x4 (&ph)[M], const u32x4 (&pl)[M],
+                                           bool& odd, f32x4 (&o)[M][TreeDims<HD>::TILES]) {
+  constexpr int N = M == 1 ? 4 : 2;
+  static_assert(TreeDims<HD>::TILES % 2 == 0, "whole groups");
+  if constexpr (TILE < TreeDims<HD>::TILES) {
+    half8_t vf[N];
+    auto decode = [&](auto i) {
+      constexpr int I = decltype(i)::value;
+      if constexpr (I < N && TILE + I < TreeDims<HD>::TILES) {
+        vf[I] = x.template vfrag<TILE + I>();
+        if constexpr (DRAFTS) vf[I] = tree_finite(vf[I], odd);
+      }
+    };
+    decode(std::integral_constant<int, 0>());
+    decode(std::integral_constant<int, 1>());
+    decode(std::integral_constant<int, 2>());
+    decode(std::integral_constant<int, 3>());
+#pragma unroll
+    for (int piece = 0; piece < 2; ++piece)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (TILE + i < TreeDims<HD>::TILES) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+            o[m][TILE + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                vf[i], __builtin_bit_cast(half8_t, piece ? ph[m] : pl[m]), o[m][TILE + i], 0, 0, 0);
+        }
+    tree_tiles<T, HD, M, DRAFTS, TILE + N>(x, ph, pl, odd, o);
+  }
+}
+
+// Two wavefronts per SIMD where the registers allow it: one's decoding and
+// exponentials run under the other's matrix instructions.
+constexpr int tree_waves_per_simd(uint32_t type, int hd, int m) {
+  return (type == T_F32 && hd * m >= 256) || (hd == 256 && (type == T_F16 || type == T_Q8_0)) || hd * m > 256 ? 1 : 2;
+}
 template <uint32_t T, int HD, int M>
-__global__ __launch_bounds__(64 * TREE_WAVES) void tree_mfma(TreeArgs a, uint32_t row_blocks) {
+__global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) void tree_mfma(TreeArgs a, uint32_t row_blocks) {
   using D = TreeDims<HD>;
   using Tile = TreeTile<T, HD>;
+  using S = TreeShared<T, HD, M>;
   constexpr bool F32 = T == T_F32;
-  constexpr uint32_t OP = HD + 4;  // LDS row of an output tile
-  __shared__ float so[TREE_WAVES][16 * OP];
-  __shared__ float sm[TREE_WAVES][M * 16], sl[TREE_WAVES][M * 16];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, c = lane & 15u, g = lane >> 4;
+  __shared__ S sh;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: the tiles' descriptors are scalars
   const uint32_t split = blockIdx.x, head = blockIdx.y / row_blocks, row0 = blockIdx.y % row_blocks * (M * 16u);
   const uint32_t G = a.qh / a.cache.kvh, rows = a.n * G, words = (a.n + 63u) / 64u;
+
+  // this lane's Q: wavefront w has row tiles w, w + 4, ..; requested before the cache's rows
+  float x[HD / 4];
+  auto ask_q = [&](int m) {
+    const uint32_t r = min(row0 + 16u * m + c, rows - 1u), i = r / G;
+    const float* const qp = a.q + (uint64_t)i * a.q_stride + ((uint64_t)head * G + (r - i * G)) * HD + g * (HD / 4);
+    tree_get_q<HD>(x, qp, a.q_vec);
+  };
+  static_assert(M <= (int)TREE_WAVES, "a row tile per wavefront");
+  if (wave < (uint32_t)M) ask_q((int)wave);
+  __builtin_amdgcn_sched_barrier(0);
+
   uint64_t hist, total;
   tree_range(a, hist, total);
-  const uint64_t tiles = (total + TREE_KEYS - 1u) / TREE_KEYS, per = (tiles + a.nsplit - 1u) / a.nsplit;
-  const uint64_t t0 = split * per, t1 = min(tiles, t0 + per);
+  const uint32_t tiles = (uint32_t)((total + TREE_KEYS - 1u) / TREE_KEYS), per = (tiles + a.nsplit - 1u) / a.nsplit;
+  const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
+  const uint32_t width = a.cache.kvh * HD;
+  const uint32_t row = T == T_F32 ? width * 4u : T == T_F16 ? width * 2u : T == T_Q8_0 ? width : width / 2u, srow = width / 16u;
+  const uint64_t sbase = a.cache.cap * (uint64_t)row;
+  Tile cur;
+  // Bounded descriptors: rows behind the last read as zeros, and nothing is
+  // read for a tile behind the last.  The loads are in no branch and in this
+  // order, here and in the loop, so that a wait for one of them (they return
+  // in order) is a wait for no later one.
+  auto rows_of = [&](uint32_t tile) { return tile < t1 ? (uint32_t)min((uint64_t)TREE_KEYS, total - (uint64_t)tile * TREE_KEYS) : 0u; };
+  auto fetch_k = [&](uint32_t tile) {
+    const uint64_t p = (uint64_t)tile * TREE_KEYS;
+    const uint32_t np = rows_of(tile);
+    cur.load_k(tree_rsrc(a.cache.k + p * row, np * row), tree_rsrc(a.cache.k + sbase + p * srow, np * srow), row, srow,
+               head, c, g);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto fetch_v = [&](uint32_t tile) {
+    const uint64_t p = (uint64_t)tile * TREE_KEYS;
+    const uint32_t np = rows_of(tile);
+    cur.load_v(tree_rsrc(a.cache.v + p * row, np * row), tree_rsrc(a.cache.v + sbase + p * srow, np * srow), row, srow,
+               head, c, g);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t tile = t0 + wave;
+  fetch_k(tile);
+  fetch_v(tile);
+  if (wave < (uint32_t)M) tree_put_q<T, HD, M>(sh, (int)wave, x, lane);
+  __syncthreads();
 
-  // this lane's rows
   uint32_t tok[M];
-  const float* qp[M];
-  float scale[M];  // score = scale * S, in powers of two
-  half8_t qh[M][D::STEPS], ql[M][D::STEPS];
-  float qf[M][F32 ? HD / 4 : 1];
-#pragma unroll
-  for (int m = 0; m < M; ++m) {
-    const uint32_t r = min(row0 + 16u * m + c, rows - 1u);
-    tok[m] = r / G;
-    qp[m] = a.q + (uint64_t)tok[m] * a.q_stride + ((uint64_t)head * G + r % G) * HD + g * (HD / 4);
-    float x[HD / 4], top = 0.f;
-#pragma unroll
-    for (int i = 0; i < HD / 4; ++i) {
-      x[i] = qp[m][i];
-      top = fmaxf(top, fabsf(x[i]));
-    }
-    float up = 1.f;
-    scale[m] = 1.44269504088896340736f / sqrtf((float)HD);
-    if constexpr (F32) {
-#pragma unroll
-      for (int i = 0; i < HD / 4; ++i) qf[m][i] = x[i];
-    } else {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (top > 0x1p-100f && top <= 3.402823466e38f) {  // to 2^10 .. 2^11
-        const uint32_t e = __float_as_uint(top) >> 23;  // biased
-        up = __uint_as_float((264u - e) << 23);         // 2^(10 - (e - 127))
-        scale[m] *= __uint_as_float((e - 10u) << 23);
-      }
-#pragma unroll
-      for (int s = 0; s < D::STEPS; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = x[8 * s + Tile::order(i)] * up;
-          qh[m][s][i] = (_Float16)y;
-          ql[m][s][i] = (_Float16)(y - (float)qh[m][s][i]);
-        }
-    }
-  }
-
+  float scale[M], ref[M], l[M];
   f32x4 o[M][D::TILES];
-  float ref[M], l[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
+    tok[m] = min(row0 + 16u * m + c, rows - 1u) / G;
+    scale[m] = sh.scale[m][c];
     ref[m] = TREE_FLOOR;
     l[m] = 0.f;
 #pragma unroll
     for (int d = 0; d < D::TILES; ++d) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const uint32_t width = a.cache.kvh * HD;
-  const uint32_t row = T == T_F32 ? width * 4u : T == T_F16 ? width * 2u : T == T_Q8_0 ? width : width / 2u, srow = width / 16u;
-  const uint64_t sbase = a.cache.cap * (uint64_t)row;
-  auto fetch = [&](Tile& x, uint64_t tile) {
-    const uint64_t p = tile * TREE_KEYS;
-    const uint32_t np = (uint32_t)min((uint64_t)TREE_KEYS, total - p);
-    x.load(tree_rsrc(a.cache.k + p * row, np * row), tree_rsrc(a.cache.k + sbase + p * srow, np * srow),
-           tree_rsrc(a.cache.v + p * row, np * row), tree_rsrc(a.cache.v + sbase + p * srow, np * srow), row, srow,
-           head, c, g);
-  };
-  // A tile ahead of the one at work; the f32 cache's long rows leave no registers for two.
-  constexpr bool AHEAD = !(F32 && HD >= 128);
-  Tile cur, nxt;
-  uint64_t tile = t0 + wave;
-  if (AHEAD && tile < t1) fetch(cur, tile);
-  for (; tile < t1; tile += TREE_WAVES) {
-    if (!AHEAD) fetch(cur, tile);
-    else if (tile + TREE_WAVES < t1) fetch(nxt, tile + TREE_WAVES);
-    __builtin_amdgcn_sched_barrier(0);
-    const uint64_t p0 = tile * TREE_KEYS;
+  auto step = [&](auto drafts) {
+    constexpr bool DRAFTS = decltype(drafts)::value;  // the tile has positions that some rows may not see
+    const uint64_t p0 = (uint64_t)tile * TREE_KEYS;
     // scores of row c at positions p0 + 16 t + 4 g + v
     f32x4 s[M][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int m = 0; m < M; ++m) s[m][0] = s[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (F32) {
 #pragma unroll
-      for (int m = 0; m < M; ++m) s[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (F32) {
+      for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-        for (int i = 0; i < HD / 4; ++i)
+        for (int m = 0; m < M; ++m) {
+          const u32x4 w = sh.q[m][i][lane];
 #pragma unroll
-          for (int m = 0; m < M; ++m)
-            s[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(cur.k[t][i]), qf[m][i], s[m][t], 0, 0, 0);
-      } else {
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < D::STEPS; ++i) {
-          const half8_t kf = cur.kfrag(t, i);
+            for (int t = 0; t < 2; ++t)
+              s[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(cur.k[t][4 * i + e]), __uint_as_float(w[e]),
+                                                              s[m][t], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < D::STEPS; ++i) {
+        const half8_t k0 = cur.kfrag(0, i), k1 = cur.kfrag(1, i);
+#pragma unroll
+        for (int piece = 0; piece < 2; ++piece)
 #pragma unroll
           for (int m = 0; m < M; ++m) {
-            s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[m][i], s[m][t], 0, 0, 0);
-            s[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[m][i], s[m][t], 0, 0, 0);
+            const half8_t qf = __builtin_bit_cast(half8_t, sh.q[m][2 * i + piece][lane]);
+            s[m][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf, s[m][0], 0, 0, 0);
+            s[m][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf, s[m][1], 0, 0, 0);
           }
-        }
       }
     }
-    const bool drafts = p0 + TREE_KEYS > hist;  // uniform
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_k(tile + TREE_WAVES);  // the old words are spent
     float p[M][8];
     uint32_t see[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      see[m] = 0xFFu;
-      if (drafts) {
-        // bits g of each half: position p0 + 16 t + 4 g + v in place 4 t + v
-        const uint32_t w = tree_window(a, words, tok[m], (int64_t)(p0 - hist), (uint32_t)(total - hist)) >> 4u * g;
-        see[m] = (w & 15u) | (w >> 12 & 0xF0u);
-      }
-      float x[8], top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = s[m][j / 4][j % 4] * scale[m];
-        if (drafts && !(see[m] >> j & 1u)) x[j] = -INFINITY;
-        top = fmaxf(top, x[j]);
-      }
-      // The reference stays until a weight would pass 2^15: few tiles rescale.
-      if (__any(top > ref[m] + TREE_MOST)) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float now = fmaxf(ref[m], top - TREE_BELOW), al = exp2f(ref[m] - now);
-        ref[m] = now;
-        l[m] *= al;
-#pragma unroll
-        for (int d = 0; d < D::TILES; ++d)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) o[m][d][v] *= al;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[m][j] = __builtin_amdgcn_exp2f(x[j] - ref[m]);
-      l[m] += ((p[m][0] + p[m][1]) + (p[m][2] + p[m][3])) + ((p[m][4] + p[m][5]) + (p[m][6] + p[m][7]));
+      see[m] = DRAFTS ? tree_places(a, words, tok[m], p0, hist, total, g) : 0xFFu;
+      tree_soften<HD, DRAFTS>(s[m], see[m], scale[m], ref[m], l[m], o[m], p[m]);
     }
-    tree_weigh<T, HD, M>(a, cur, p, see, drafts, p0, total, head, c, g, so[wave], o);
-    if (AHEAD) cur = nxt;
-  }
+    bool odd = false;
+    if constexpr (F32) {
+#pragma unroll
+      for (int d = 0; d < D::TILES; ++d)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float v = __uint_as_float(cur.v[j][d]);
+          if (DRAFTS && !(fabsf(v) <= 3.402823466e38f)) {
+            odd = true;
+            v = 0.f;
+          }
+#pragma unroll
+          for (int m = 0; m < M; ++m) o[m][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[m][j], o[m][d], 0, 0, 0);
+        }
+    } else {
+      u32x4 ph[M], pl[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t h, r;
+          tree_pieces(p[m][2 * j], p[m][2 * j + 1], h, r);
+          ph[m][j] = h;
+          pl[m][j] = r;
+        }
+      tree_tiles<T, HD, M, DRAFTS, 0>(cur, ph, pl, odd, o);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_v(tile + TREE_WAVES);
+    if (DRAFTS && __any(odd)) tree_odd_rows<HD, M>(a, p, see, p0, total, head, c, g, sh.sum[wave], o);
+  };
+  // the drafts come last
+  for (; tile < t1 && (uint64_t)tile * TREE_KEYS + TREE_KEYS <= hist; tile += TREE_WAVES) step(std::false_type());
+  for (; tile < t1; tile += TREE_WAVES) step(std::true_type());
 
-  // join the wavefronts, a row tile at a time
+  // join the wavefronts, a row tile (and 128 dims) at a time
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     l[m] += __shfl_xor(l[m], 16);
     l[m] += __shfl_xor(l[m], 32);
     if (g == 0) {
-      sm[wave][16 * m + c] = ref[m];
-      sl[wave][16 * m + c] = l[m];
+      sh.m[wave][16 * m + c] = ref[m];
+      sh.l[wave][16 * m + c] = l[m];
     }
   }
 #pragma unroll
   for (int m = 0; m < M; ++m) {
-    __syncthreads();
-    float top = TREE_FLOOR;
 #pragma unroll
-    for (uint32_t w = 0; w < TREE_WAVES; ++w) top = fmaxf(top, sm[w][16 * m + c]);
-    const float al = exp2f(ref[m] - top);
+    for (uint32_t part = 0; part < S::PARTS; ++part) {
+      __syncthreads();
+      float top = TREE_FLOOR;
 #pragma unroll
-    for (int d = 0; d < D::TILES; ++d)
+      for (uint32_t w = 0; w < TREE_WAVES; ++w) top = fmaxf(top, sh.m[w][16 * m + c]);
+      const float al = exp2f(ref[m] - top);
 #pragma unroll
-      for (uint32_t v = 0; v < 4; ++v) so[wave][c * OP + D::dim(d, 4u * g + v)] = o[m][d][v] * al;
-    __syncthreads();
-    for (uint32_t e = tid; e < 16u * HD / 4u; e += 64u * TREE_WAVES) {
-      const uint32_t rr = e / (HD / 4u), d = e % (HD / 4u) * 4u, r = row0 + 16u * m + rr;
-      if (r >= rows) continue;
-      float best = TREE_FLOOR, sum = 0.f;
+      for (int d = 0; d < D::TILES; ++d)
 #pragma unroll
-      for (uint32_t w = 0; w < TREE_WAVES; ++w) best = fmaxf(best, sm[w][16 * m + rr]);
+        for (uint32_t v = 0; v < 4; ++v) {
+          const uint32_t dim = D::dim(d, 4u * g + v);
+          if (S::PARTS == 1 || dim / S::CH == part) sh.sum[wave][c * S::OP + dim % S::CH] = o[m][d][v] * al;
+        }
+      __syncthreads();
+      for (uint32_t e = tid; e < 16u * S::CH / 4u; e += 64u * TREE_WAVES) {
+        const uint32_t rr = e / (S::CH / 4u), dd = e % (S::CH / 4u) * 4u, d = part * S::CH + dd, r = row0 + 16u * m + rr;
+        if (r >= rows) continue;
+        float best = TREE_FLOOR, sum = 0.f;
 #pragma unroll
-      for (uint32_t w = 0; w < TREE_WAVES; ++w) sum += sl[w][16 * m + rr] * exp2f(sm[w][16 * m + rr] - best);
-      float4 y = *reinterpret_cast<const float4*>(&so[0][rr * OP + d]);
+        for (uint32_t w = 0; w < TREE_WAVES; ++w) best = fmaxf(best, sh.m[w][16 * m + rr]);
 #pragma unroll
-      for (uint32_t w = 1; w < TREE_WAVES; ++w) {
-        const float4 z = *reinterpret_cast<const float4*>(&so[w][rr * OP + d]);
-        y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-      }
-      const uint32_t i = r / G, h = head * G + r % G;
-      if (a.nsplit == 1) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        float* const out = a.out + (uint64_t)i * a.out_stride + (uint64_t)h * HD + d;
-        out[0] = y.x * inv; out[1] = y.y * inv; out[2] = y.z * inv; out[3] = y.w * inv;
-      } else {
-        float* const rec = a.ws + (((uint64_t)split * a.n + i) * a.qh + h) * (HD + 4);
-        *reinterpret_cast<float4*>(rec + d) = y;
-        if (d == 0) { rec[HD] = best; rec[HD + 1] = sum; }
+        for (uint32_t w = 0; w < TREE_WAVES; ++w) sum += sh.l[w][16 * m + rr] * exp2f(sh.m[w][16 * m + rr] - best);
+        float4 y = *reinterpret_cast<const float4*>(&sh.sum[0][rr * S::OP + dd]);
+#pragma unroll
+        for (uint32_t w = 1; w < TREE_WAVES; ++w) {
+          const float4 z = *reinterpret_cast<const float4*>(&sh.sum[w][rr * S::OP + dd]);
+          y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+        }
+        const uint32_t i = r / G, h = head * G + r % G;
+        if (a.nsplit == 1) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          float* const out = a.out + (uint64_t)i * a.out_stride + (uint64_t)h * HD + d;
+          out[0] = y.x * inv; out[1] = y.y * inv; out[2] = y.z * inv; out[3] = y.w * inv;
+        } else {
+          float* const rec = a.ws + (((uint64_t)split * a.n + i) * a.qh + h) * (HD + 4);
+          *reinterpret_cast<float4*>(rec + d) = y;
+          if (d == 0) { rec[HD] = best; rec[HD + 1] = sum; }
+        }
       }
     }
   }
 }
 
-// Joins a row's records: HD / 4 lanes of 4 dims per row.
+// ------------------------------------------- rows over the wavefronts
+
+// With many rows the decoding is what a wavefront does most: here the four
+// wavefronts of a workgroup have rows of their own (M tiles of 16 each) and the
+// same positions, each decodes a quarter of a tile into LDS as the matrix
+// instructions take it, and all read it from there.  Tiles are double-buffered:
+// one barrier each; the words of the next but one are in flight.
+//   Wavefront w decodes, of K, half tile w % 2 and steps from w / 2 (STEPS / 2
+//   rounded up), and of V its positions 4 t + v = 2 w, 2 w + 1 for all dims:
+//   word w of every tile's operand.
+template <uint32_t T, int HD> struct TreePart {
+  using Tile = TreeTile<T, HD>;
+  using D = TreeDims<HD>;
+  static constexpr int KSTEPS = (D::STEPS + 1) / 2, SW = Tile::BITS / 4;  // steps, words of a step
+  uint32_t k[KSTEPS * SW], ks[KSTEPS], v[2][Tile::VW], vs[2][2];
+
+  __device__ __forceinline__ void load_k(TreeRsrc kr, TreeRsrc ksr, uint32_t row, uint32_t srow, uint32_t head,
+                                         uint32_t c, uint32_t g, uint32_t wave) {
+    const uint32_t p = 16u * (wave & 1u) + c, s0 = (wave >> 1) * KSTEPS;
+    tree_words<KSTEPS * SW>(k, kr, p * row + head * (HD * Tile::BITS / 8) + g * (D::STEPS * SW * 4u) + s0 * (SW * 4u));
+    if constexpr (Tile::QUANT) {
+#pragma unroll
+      for (int i = 0; i < KSTEPS; ++i)
+        if (i == 0 || HD == 96)  // elsewhere a wavefront's steps lie in one block
+          ks[i] = tree_u16(ksr, p * srow + head * (HD / 16) + 2u * ((g * (HD / 4) + 8u * (s0 + i)) / 32u));
+    }
+  }
+  __device__ __forceinline__ void load_v(TreeRsrc vr, TreeRsrc vsr, uint32_t row, uint32_t srow, uint32_t head,
+                                         uint32_t c, uint32_t g, uint32_t wave) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const uint32_t j = 2u * wave + i, p = 16u * (j / 4u) + 4u * g + j % 4u, hb = head * (HD * Tile::BITS / 8);
+      tree_bytes<Tile::B0>(v[i], vr, p * row + hb + c * Tile::B0);
+      if constexpr (Tile::B1 > 0) tree_bytes<Tile::B1>(v[i] + Tile::VW0, vr, p * row + hb + 16u * Tile::B0 + c * Tile::B1);
+      if constexpr (Tile::QUANT) {
+        vs[i][0] = tree_u16(vsr, p * srow + head * (HD / 16) + 2u * (c * D::W0 / 32u));
+        if constexpr (Tile::VS == 2) vs[i][1] = tree_u16(vsr, p * srow + head * (HD / 16) + 4u);
+      }
+    }
+  }
+  __device__ __forceinline__ half8_t kfrag(int s) const {
+    u32x4 w;
+    if constexpr (T == T_F16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = k[4 * s + i];
+    } else {
+      Tile::decode_k(k + s * SW, ks[HD == 96 ? s : 0], w);
+    }
+    return __builtin_bit_cast(half8_t, w);
+  }
+};
+
+template <int HD> struct TreeRowsShared {
+  u32x4 k[2][2][TreeDims<HD>::STEPS][64];  // buffer, half tile, step, lane
+  u32x4 v[2][TreeDims<HD>::TILES][64];
+  float odd[TREE_WAVES][16 * TREE_ODD];
+};
+
+template <uint32_t T, int HD, int M>
+__global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a, uint32_t row_blocks) {
+  using D = TreeDims<HD>;
+  using Tile = TreeTile<T, HD>;
+  using Part = TreePart<T, HD>;
+  __shared__ TreeRowsShared<HD> sh;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t split = blockIdx.x, head = blockIdx.y / row_blocks;
+  const uint32_t row0 = (blockIdx.y % row_blocks * TREE_WAVES + wave) * (M * 16u);
+  const uint32_t G = a.qh / a.cache.kvh, rows = a.n * G, words = (a.n + 63u) / 64u;
+  uint64_t hist, total;
+  tree_range(a, hist, total);
+  const uint32_t tiles = (uint32_t)((total + TREE_KEYS - 1u) / TREE_KEYS), per = (tiles + a.nsplit - 1u) / a.nsplit;
+  const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
+  const uint32_t width = a.cache.kvh * HD;
+  const uint32_t row = T == T_F16 ? width * 2u : T == T_Q8_0 ? width : width / 2u, srow = width / 16u;
+  const uint64_t sbase = a.cache.cap * (uint64_t)row;
+  Part part;
+  auto fetch = [&](uint32_t tile) {  // as in tree_mfma: in no branch
+    const uint64_t p = (uint64_t)tile * TREE_KEYS;
+    const uint32_t np = tile < t1 ? (uint32_t)min((uint64_t)TREE_KEYS, total - p) : 0u;
+    part.load_k(tree_rsrc(a.cache.k + p * row, np * row), tree_rsrc(a.cache.k + sbase + p * srow, np * srow), row, srow,
+                head, c, g, wave);
+    part.load_v(tree_rsrc(a.cache.v + p * row, np * row), tree_rsrc(a.cache.v + sbase + p * srow, np * srow), row, srow,
+                head, c, g, wave);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto put = [&](uint32_t buf) {
+    const uint32_t t = wave & 1u, s0 = (wave >> 1) * Part::KSTEPS;
+#pragma unroll
+    for (int i = 0; i < Part::KSTEPS; ++i)
+      if (D::STEPS % 2 == 0 || s0 + i < (uint32_t)D::STEPS) sh.k[buf][t][s0 + i][lane] = __builtin_bit_cast(u32x4, part.kfrag(i));
+    uint32_t w[D::TILES];
+    Tile::decode_v(part.v[0], part.v[1], part.vs[0], part.vs[1], w);
+#pragma unroll
+    for (int d = 0; d < D::TILES; ++d) reinterpret_cast<uint32_t*>(&sh.v[buf][d][lane])[wave] = w[d];
+  };
+
+  half8_t qh[M][D::STEPS], ql[M][D::STEPS];
+  uint32_t tok[M];
+  float scale[M], ref[M], l[M];
+  f32x4 o[M][D::TILES];
+  float x[M][HD / 4];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const uint32_t r = min(row0 + 16u * m + c, rows - 1u);
+    tok[m] = r / G;
+    const float* const qp = a.q + (uint64_t)tok[m] * a.q_stride + ((uint64_t)head * G + (r - tok[m] * G)) * HD + g * (HD / 4);
+    tree_get_q<HD>(x[m], qp, a.q_vec);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  fetch(t0);
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    scale[m] = tree_split_q<T, HD>(x[m], [&](int s, int piece, u32x4 w) {
+      (piece ? qh : ql)[m][s] = __builtin_bit_cast(half8_t, w);
+    });
+    ref[m] = TREE_FLOOR;
+    l[m] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D::TILES; ++d) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  put(0);
+  fetch(t0 + 1);
+  __syncthreads();
+
+  auto step = [&](auto drafts, uint32_t tile, uint32_t buf) {
+    constexpr bool DRAFTS = decltype(drafts)::value;
+    const uint64_t p0 = (uint64_t)tile * TREE_KEYS;
+    f32x4 s[M][2];
+#pragma unroll
+    for (int m = 0; m < M; ++m) s[m][0] = s[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D::STEPS; ++i) {
+      const half8_t k0 = __builtin_bit_cast(half8_t, sh.k[buf][0][i][lane]), k1 = __builtin_bit_cast(half8_t, sh.k[buf][1][i][lane]);
+#pragma unroll
+      for (int piece = 0; piece < 2; ++piece)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          s[m][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, piece ? qh[m][i] : ql[m][i], s[m][0], 0, 0, 0);
+          s[m][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, piece ? qh[m][i] : ql[m][i], s[m][1], 0, 0, 0);
+        }
+    }
+    float p[M][8];
+    uint32_t see[M];
+    u32x4 ph[M], pl[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      see[m] = DRAFTS ? tree_places(a, words, tok[m], p0, hist, total, g) : 0xFFu;
+      tree_soften<HD, DRAFTS>(s[m], see[m], scale[m], ref[m], l[m], o[m], p[m]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t h, r;
+        tree_pieces(p[m][2 * j], p[m][2 * j + 1], h, r);
+        ph[m][j] = h;
+        pl[m][j] = r;
+      }
+    }
+    bool odd = false;
+    constexpr int N = M == 1 ? 4 : 2;
+#pragma unroll
+    for (int d = 0; d < D::TILES; d += N) {
+      half8_t vf[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (d + i < D::TILES) {
+          vf[i] = __builtin_bit_cast(half8_t, sh.v[buf][d + i][lane]);
+          if (DRAFTS) vf[i] = tree_finite(vf[i], odd);
+        }
+#pragma unroll
+      for (int piece = 0; piece < 2; ++piece)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (d + i < D::TILES) {
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+              o[m][d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], __builtin_bit_cast(half8_t, piece ? ph[m] : pl[m]),
+                                                                    o[m][d + i], 0, 0, 0);
+          }
+    }
+    if (DRAFTS && __any(odd)) tree_odd_rows<HD, M>(a, p, see, p0, total, head, c, g, sh.odd[wave], o);
+    put(buf ^ 1u);
+    fetch(tile + 2u);
+    __syncthreads();
+  };
+  uint32_t buf = 0, tile = t0;
+  for (; tile < t1 && (uint64_t)tile * TREE_KEYS + TREE_KEYS <= hist; ++tile, buf ^= 1u) step(std::false_type(), tile, buf);
+  for (; tile < t1; ++tile, buf ^= 1u) step(std::true_type(), tile, buf);
+
+  // each wavefront has its rows alone
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    l[m] += __shfl_xor(l[m], 16);
+    l[m] += __shfl_xor(l[m], 32);
+    const uint32_t r = row0 + 16u * m + c;
+    if (r >= rows) continue;
+    const uint32_t h = head * G + (r - tok[m] * G);
+    const bool whole = a.nsplit == 1;
+    const float inv = whole ? (l[m] == 0.f ? 0.f : 1.f / l[m]) : 1.f;
+    float* const rec = a.ws + (((uint64_t)split * a.n + tok[m]) * a.qh + h) * (HD + 4);
+    float* const out = whole ? a.out + (uint64_t)tok[m] * a.out_stride + (uint64_t)h * HD : rec;
+#pragma unroll
+    for (int d = 0; d < D::TILES; d += D::W1 ? 2 : 4)
+#pragma unroll
+      for (uint32_t v = 0; v < 4; ++v) {
+        constexpr int N = D::W1 ? 2 : 4;  // consecutive tiles are consecutive dims
+        float* const to = out + D::dim(d, 4u * g + v);
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) to[i] = o[m][d + i][v] * inv;
+        } else if constexpr (N == 4) {
+          *reinterpret_cast<float4*>(to) = make_float4(o[m][d][v], o[m][d + 1][v], o[m][d + 2][v], o[m][d + 3][v]);
+        } else {
+          *reinterpret_cast<float2*>(to) = make_float2(o[m][d][v], o[m][d + 1][v]);
+        }
+      }
+    if (!whole && g == 0) {
+      rec[HD] = ref[m];
+      rec[HD + 1] = l[m];
+    }
+  }
+}
+
+// Joins a row's records: HD / 4 lanes of 4 dims take every JOIN-th split, and
+// their sums meet in LDS, so that a row of many splits is a few loads deep.
 template <int HD>
 __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
-  constexpr uint32_t LANES = HD / 4, PER = 256u / LANES;
-  const uint64_t rows = (uint64_t)a.n * a.qh, r = (uint64_t)blockIdx.x * PER + threadIdx.x / LANES;
-  const uint32_t d = threadIdx.x % LANES * 4u;
-  if (threadIdx.x >= LANES * PER || r >= rows) return;
+  constexpr uint32_t LANES = HD / 4, JOIN = 256u / LANES;
+  __shared__ __align__(16) float y[JOIN][HD + 4];
+  const uint64_t rows = (uint64_t)a.n * a.qh, r = blockIdx.x;
+  const uint32_t part = threadIdx.x / LANES, d = threadIdx.x % LANES * 4u;
   const float* const rec = a.ws + r * (HD + 4);
   const uint64_t step = rows * (HD + 4);
-  float top = TREE_FLOOR;
-  for (uint32_t s = 0; s < a.nsplit; ++s) top = fmaxf(top, rec[s * step + HD]);
-  float sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+  if (part < JOIN) {
+    float top = TREE_FLOOR, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (uint32_t s = 0; s < a.nsplit; ++s) {
-    const float w = exp2f(rec[s * step + HD] - top);
-    sum = fmaf(rec[s * step + HD + 1], w, sum);
-    const float4 z = *reinterpret_cast<const float4*>(rec + s * step + d);
-    y[0] = fmaf(z.x, w, y[0]); y[1] = fmaf(z.y, w, y[1]); y[2] = fmaf(z.z, w, y[2]); y[3] = fmaf(z.w, w, y[3]);
+    for (uint32_t s = part; s < a.nsplit; s += JOIN) {
+      const float* const at = rec + s * step;
+      const float4 z = *reinterpret_cast<const float4*>(at + d);
+      const float m = at[HD], now = fmaxf(top, m), al = exp2f(top - now), w = exp2f(m - now);
+      top = now;
+      sum = fmaf(sum, al, at[HD + 1] * w);
+      o[0] = fmaf(o[0], al, z.x * w); o[1] = fmaf(o[1], al, z.y * w);
+      o[2] = fmaf(o[2], al, z.z * w); o[3] = fmaf(o[3], al, z.w * w);
+    }
+    *reinterpret_cast<float4*>(&y[part][d]) = make_float4(o[0], o[1], o[2], o[3]);
+    if (d == 0) { y[part][HD] = top; y[part][HD + 1] = sum; }
+  }
+  __syncthreads();
+  if (part != 0) return;
+  float top = TREE_FLOOR, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (uint32_t p = 0; p < JOIN; ++p) top = fmaxf(top, y[p][HD]);
+#pragma unroll
+  for (uint32_t p = 0; p < JOIN; ++p) {
+    const float w = exp2f(y[p][HD] - top);
+    const float4 z = *reinterpret_cast<const float4*>(&y[p][d]);
+    sum = fmaf(y[p][HD + 1], w, sum);
+    o[0] = fmaf(z.x, w, o[0]); o[1] = fmaf(z.y, w, o[1]); o[2] = fmaf(z.z, w, o[2]); o[3] = fmaf(z.w, w, o[3]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   float* const out = a.out + r / a.qh * a.out_stride + r % a.qh * HD + d;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = y[e] * inv;
+  for (int e = 0; e < 4; ++e) out[e] = o[e] * inv;
 }
 
 // ---------------------------------------------------------------- launches
 
 static bool tree_on_matrix_cores(uint32_t hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
-// Row tiles of a wavefront: a decoded tile serves more rows with two.  With
-// head_dim 256 the second tile's registers do not fit.
-static uint32_t tree_row_tiles(uint64_t rows, uint32_t hd) { return rows > 16 && hd <= 128 ? 2 : 1; }
+// The kernel of a shape: few rows go to tree_mfma, whose wavefronts split the
+// positions (tiles: row tiles of each), more to tree_rows, whose wavefronts
+// split the rows.
+struct TreePlan {
+  bool rows_apart;
+  uint32_t tiles, block_rows;  // row tiles of a wavefront, rows of a workgroup
+};
+static TreePlan tree_plan(uint64_t rows, uint32_t hd, uint32_t type) {
+  TreePlan p{rows > 32 && type != T_F32, 1, 16};
+  if (p.rows_apart) {
+    p.tiles = rows > 64 && hd != 256 ? 2 : 1;
+    p.block_rows = 16 * TREE_WAVES * p.tiles;
+  } else {
+    p.tiles = rows > 16 && hd != 256 ? 2 : 1;
+    p.block_rows = 16 * p.tiles;
+  }
+  return p;
+}
 
-uint32_t tree_splits(uint64_t total, uint32_t n, uint32_t qh, uint32_t kvh, uint32_t hd, uint32_t) {
+uint32_t tree_splits(uint64_t total, uint32_t n, uint32_t qh, uint32_t kvh, uint32_t hd, uint32_t type) {
   if (!tree_on_matrix_cores(hd)) return 1;
-  const uint64_t rows = (uint64_t)n * (qh / kvh), per = 16u * tree_row_tiles(rows, hd);
-  const uint64_t units = kvh * ((rows + per - 1) / per), tiles = (total + TREE_KEYS - 1) / TREE_KEYS;
-  const uint64_t want = (512 + units - 1) / units, most = (tiles + TREE_WAVES - 1) / TREE_WAVES;
-  const uint64_t s = want < most ? want : most;
+  const uint64_t rows = (uint64_t)n * (qh / kvh);
+  const TreePlan p = tree_plan(rows, hd, type);
+  const uint64_t units = kvh * ((rows + p.block_rows - 1) / p.block_rows), tiles = (total + TREE_KEYS - 1) / TREE_KEYS;
+  const uint64_t want = (512 + units - 1) / units, least = p.rows_apart ? 4 : TREE_WAVES;  // tiles of a split
+  const uint64_t most = (tiles + least - 1) / least, s = want < most ? want : most;
   return (uint32_t)(s ? s : 1);
 }
 uint64_t tree_ws_floats(uint32_t nsplit, uint32_t n, uint32_t qh, uint32_t hd) {
   return nsplit > 1 ? (uint64_t)nsplit * n * qh * (hd + 4) : 0;
 }
 
-template <uint32_t T, int HD, int M>
+template <uint32_t T, int HD>
 static void launch_tree(const TreeArgs& a, hipStream_t st) {
   const uint64_t rows = (uint64_t)a.n * (a.qh / a.cache.kvh);
-  const uint32_t blocks = (uint32_t)((rows + 16 * M - 1) / (16 * M));
-  RF_KLAUNCH((tree_mfma<T, HD, M>), dim3(a.nsplit, a.cache.kvh * blocks), dim3(64 * TREE_WAVES), 0, st, a, blocks);
-  if (a.nsplit > 1) {
-    const uint64_t all = (uint64_t)a.n * a.qh;
-    constexpr uint32_t PER = 256 / (HD / 4);
-    RF_KLAUNCH(tree_join<HD>, dim3((uint32_t)((all + PER - 1) / PER)), dim3(256), 0, st, a);
+  const TreePlan p = tree_plan(rows, HD, T);
+  const uint32_t blocks = (uint32_t)((rows + p.block_rows - 1) / p.block_rows);
+  const dim3 grid(a.nsplit, a.cache.kvh * blocks), wg(64 * TREE_WAVES);
+  if (p.rows_apart) {
+    if constexpr (T != T_F32) {
+      if constexpr (HD <= 128) {
+        if (p.tiles == 2) RF_KLAUNCH((tree_rows<T, HD, 2>), grid, wg, 0, st, a, blocks);
+      }
+      if (p.tiles == 1) RF_KLAUNCH((tree_rows<T, HD, 1>), grid, wg, 0, st, a, blocks);
+    }
+  } else {
+    if constexpr (HD <= 128) {
+      if (p.tiles == 2) RF_KLAUNCH((tree_mfma<T, HD, 2>), grid, wg, 0, st, a, blocks);
+    }
+    if (p.tiles == 1) RF_KLAUNCH((tree_mfma<T, HD, 1>), grid, wg, 0, st, a, blocks);
   }
+  if (a.nsplit > 1) RF_KLAUNCH(tree_join<HD>, dim3(a.n * a.qh), dim3(256), 0, st, a);
 }
 
 template <uint32_t T>
 static void launch_tree_type(const TreeArgs& a, hipStream_t st) {
-  const bool two = tree_row_tiles((uint64_t)a.n * (a.qh / a.cache.kvh), a.cache.hd) == 2;
   switch (a.cache.hd) {
-    case 64: two ? launch_tree<T, 64, 2>(a, st) : launch_tree<T, 64, 1>(a, st); break;
-    case 96: two ? launch_tree<T, 96, 2>(a, st) : launch_tree<T, 96, 1>(a, st); break;
-    case 128: two ? launch_tree<T, 128, 2>(a, st) : launch_tree<T, 128, 1>(a, st); break;
-    default: launch_tree<T, 256, 1>(a, st);
+    case 64: launch_tree<T, 64>(a, st); break;
+    case 96: launch_tree<T, 96>(a, st); break;
+    case 128: launch_tree<T, 128>(a, st); break;
+    default: launch_tree<T, 256>(a, st);
   }
 }
 
