@@ -525,32 +525,43 @@ def kv_cache_bytes(ggml_type: int, capacity: int, n_kv_heads: int, head_dim: int
     return int(_lib.load().rf_kv_cache_bytes(ggml_type, capacity, n_kv_heads, head_dim))
 
 
-def _span(n: int, width: int, stride: int) -> int:
-    """Bytes that n rows of width floats, stride apart, reach over."""
-    return 4 * ((n - 1) * (stride or width) + width) if n else 0
+def _rows_arg(op: str, name: str, a, n: int = 1, width: int = 1, stride: int = 0, size: int = 4):
+    """The address of n rows of width elements (size bytes each), stride elements apart; a DeviceArray must hold
+    them, an address is taken as it is."""
+    if type(a) is int or a is None:
+        return a
+    p = _ptr(a)
+    if isinstance(a, DeviceArray):
+        need = size * ((n - 1) * (stride or width) + width) if n else 0
+        if a.nbytes < need:
+            raise RamforgeError(_lib.RF_ERR_INVALID,
+                                f"{op} shape mismatch: {name} holds {a.nbytes} bytes, {need} needed")
+    return p
 
 
 def kv_store(ctx: Context, cache: KvCache, k, v, first: int, n: int, k_stride: int = 0, v_stride: int = 0,
              stream=None) -> None:
     """n rows of k and v ([n_kv_heads][head_dim] f32, strides in floats) into cache positions first .. first + n - 1."""
-    _fits("KV store", k=(k, _span(n, cache.width, k_stride)), v=(v, _span(n, cache.width, v_stride)))
-    _lib.check(ctx.lib.rf_kv_store(ctx.handle, cache.ref, _ptr(k), k_stride, _ptr(v), v_stride, first, n, stream))
+    k = _rows_arg("KV store", "k", k, n, cache.width, k_stride)
+    v = _rows_arg("KV store", "v", v, n, cache.width, v_stride)
+    _lib.check(ctx.lib.rf_kv_store(ctx.handle, cache.ref, k, k_stride, v, v_stride, first, n, stream))
 
 
 def kv_load(ctx: Context, cache: KvCache, first: int, n: int, k, v, k_stride: int = 0, v_stride: int = 0,
             stream=None) -> None:
     """Cache positions first .. first + n - 1 as rows of k and v (f32)."""
-    _fits("KV load", k=(k, _span(n, cache.width, k_stride)), v=(v, _span(n, cache.width, v_stride)))
-    _lib.check(ctx.lib.rf_kv_load(ctx.handle, cache.ref, first, n, _ptr(k), k_stride, _ptr(v), v_stride, stream))
+    k = _rows_arg("KV load", "k", k, n, cache.width, k_stride)
+    v = _rows_arg("KV load", "v", v, n, cache.width, v_stride)
+    _lib.check(ctx.lib.rf_kv_load(ctx.handle, cache.ref, first, n, k, k_stride, v, v_stride, stream))
 
 
 def kv_move(ctx: Context, caches, src, first: int, n: int, stream=None) -> None:
     """In each cache (a KvCacheList, or a sequence of KvCache) positions first + j take what positions src[j] (device
     uint32) held before: an accepted path of drafts moves to the end of the history."""
-    if not isinstance(caches, KvCacheList):
+    if type(caches) is not KvCacheList:
         caches = KvCacheList(caches)
-    _fits("KV move", src=(src, 4 * n))
-    _lib.check(ctx.lib.rf_kv_move(ctx.handle, caches.ref, caches.n, _ptr(src), first, n, stream))
+    src = _rows_arg("KV move", "src", src, n)
+    _lib.check(ctx.lib.rf_kv_move(ctx.handle, caches.ref, caches.n, src, first, n, stream))
 
 
 def qk_norm_rope(ctx: Context, q, k, q_norm, k_norm, eps: float, positions, n_tokens: int, n_heads: int,
@@ -558,13 +569,17 @@ def qk_norm_rope(ctx: Context, q, k, q_norm, k_norm, eps: float, positions, n_to
                  q_out_stride: int = 0, k_out_stride: int = 0, stream=None) -> None:
     """RMS norm of every query and key head (weights None: no norm) and half-split RoPE at positions[t] (device
     uint32), n_tokens rows in one pass."""
-    qd, kvd = n_heads * head_dim, n_kv_heads * head_dim
-    _fits("QK norm and RoPE", q=(q, _span(n_tokens, qd, q_stride)), k=(k, _span(n_tokens, kvd, k_stride)),
-          q_norm=(q_norm, 4 * head_dim), k_norm=(k_norm, 4 * head_dim), positions=(positions, 4 * n_tokens),
-          q_out=(q_out, _span(n_tokens, qd, q_out_stride)), k_out=(k_out, _span(n_tokens, kvd, k_out_stride)))
-    _lib.check(ctx.lib.rf_qk_norm_rope(ctx.handle, _ptr(q), q_stride, _ptr(k), k_stride, _ptr(q_norm), _ptr(k_norm),
-                                       eps, _ptr(positions), n_tokens, n_heads, n_kv_heads, head_dim, freq_base,
-                                       _ptr(q_out), q_out_stride, _ptr(k_out), k_out_stride, stream))
+    op, n, qd, kvd = "QK norm and RoPE", n_tokens, n_heads * head_dim, n_kv_heads * head_dim
+    q = _rows_arg(op, "q", q, n, qd, q_stride)
+    k = _rows_arg(op, "k", k, n, kvd, k_stride)
+    q_norm = _rows_arg(op, "q_norm", q_norm, head_dim)
+    k_norm = _rows_arg(op, "k_norm", k_norm, head_dim)
+    positions = _rows_arg(op, "positions", positions, n)
+    q_out = _rows_arg(op, "q_out", q_out, n, qd, q_out_stride)
+    k_out = _rows_arg(op, "k_out", k_out, n, kvd, k_out_stride)
+    _lib.check(ctx.lib.rf_qk_norm_rope(ctx.handle, q, q_stride, k, k_stride, q_norm, k_norm, eps, positions, n,
+                                       n_heads, n_kv_heads, head_dim, freq_base, q_out, q_out_stride, k_out,
+                                       k_out_stride, stream))
 
 
 def qk_norm_rope_store(ctx: Context, q, k, v, q_norm, k_norm, eps: float, positions, n_tokens: int, n_heads: int,
@@ -572,22 +587,27 @@ def qk_norm_rope_store(ctx: Context, q, k, v, q_norm, k_norm, eps: float, positi
                        v_stride: int = 0, q_out_stride: int = 0, stream=None) -> None:
     """qk_norm_rope with the rotated k and the rows v written into cache positions first .. in the same pass
     (positions None: the cache positions)."""
-    qd, kvd = n_heads * cache.head_dim, cache.width
-    _fits("QK norm and RoPE store", q=(q, _span(n_tokens, qd, q_stride)), k=(k, _span(n_tokens, kvd, k_stride)),
-          v=(v, _span(n_tokens, kvd, v_stride)), q_norm=(q_norm, 4 * cache.head_dim),
-          k_norm=(k_norm, 4 * cache.head_dim), positions=(positions, 4 * n_tokens),
-          q_out=(q_out, _span(n_tokens, qd, q_out_stride)))
-    _lib.check(ctx.lib.rf_qk_norm_rope_store(ctx.handle, _ptr(q), q_stride, _ptr(k), k_stride, _ptr(v), v_stride,
-                                             _ptr(q_norm), _ptr(k_norm), eps, _ptr(positions), n_tokens, n_heads,
-                                             freq_base, _ptr(q_out), q_out_stride, cache.ref, first, stream))
+    op, n, qd, kvd = "QK norm and RoPE store", n_tokens, n_heads * cache.head_dim, cache.width
+    q = _rows_arg(op, "q", q, n, qd, q_stride)
+    k = _rows_arg(op, "k", k, n, kvd, k_stride)
+    v = _rows_arg(op, "v", v, n, kvd, v_stride)
+    q_norm = _rows_arg(op, "q_norm", q_norm, cache.head_dim)
+    k_norm = _rows_arg(op, "k_norm", k_norm, cache.head_dim)
+    positions = _rows_arg(op, "positions", positions, n)
+    q_out = _rows_arg(op, "q_out", q_out, n, qd, q_out_stride)
+    _lib.check(ctx.lib.rf_qk_norm_rope_store(ctx.handle, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm, eps,
+                                             positions, n, n_heads, freq_base, q_out, q_out_stride, cache.ref, first,
+                                             stream))
 
 
 def tree_mask(ctx: Context, parents, n: int, base: int, mask, positions=None, length=None, stream=None) -> None:
     """The ancestor mask ([n][ceil(n / 64)] uint64) of a tree of n drafted tokens from their parents (device int32,
     -1: the history), and their positions, base plus depth (uint32)."""
-    _fits("tree mask", parents=(parents, 4 * n), mask=(mask, 8 * n * ((n + 63) // 64)), positions=(positions, 4 * n))
-    _lib.check(ctx.lib.rf_tree_mask(ctx.handle, _ptr(parents), n, base, _ptr(length), _ptr(mask), _ptr(positions),
-                                    stream))
+    parents = _rows_arg("tree mask", "parents", parents, n)
+    mask = _rows_arg("tree mask", "mask", mask, n, (n + 63) // 64, 0, 8)
+    positions = _rows_arg("tree mask", "positions", positions, n)
+    _lib.check(ctx.lib.rf_tree_mask(ctx.handle, parents, n, base, _rows_arg("tree mask", "length", length), mask,
+                                    positions, stream))
 
 
 def attention_tree(ctx: Context, q, cache: KvCache, hist_len: int, n: int, n_heads: int, mask=None,
@@ -595,13 +615,14 @@ def attention_tree(ctx: Context, q, cache: KvCache, hist_len: int, n: int, n_hea
                    stream=None) -> DeviceArray:
     """Attention of n tokens at cache positions hist_len .. hist_len + n - 1, over the history and what their mask
     rows allow of one another (mask None: a chain)."""
-    qd = n_heads * cache.head_dim
-    _fits("tree attention", q=(q, _span(n, qd, q_stride)), out=(out, _span(n, qd, out_stride)),
-          mask=(mask, 8 * n * ((n + 63) // 64)))
+    op, qd = "tree attention", n_heads * cache.head_dim
     if out is None:
-        out = ctx.empty((n, qd) if out_stride in (0, qd) else (n, out_stride))
-    _lib.check(ctx.lib.rf_attention_tree(ctx.handle, _ptr(q), q_stride, cache.ref, hist_len, _ptr(mask), n, n_heads,
-                                         _ptr(out), out_stride, stream))
+        out = ctx.empty((n, out_stride or qd))
+    q = _rows_arg(op, "q", q, n, qd, q_stride)
+    mask = _rows_arg(op, "mask", mask, n, (n + 63) // 64, 0, 8)
+    to = _rows_arg(op, "out", out, n, qd, out_stride)
+    _lib.check(ctx.lib.rf_attention_tree(ctx.handle, q, q_stride, cache.ref, hist_len, mask, n, n_heads, to,
+                                         out_stride, stream))
     return out
 
 

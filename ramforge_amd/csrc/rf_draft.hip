@@ -220,7 +220,7 @@ uint64_t rf_attention_tree_workspace_bytes(uint64_t max_positions, uint64_t n, u
   if (max_positions == 0 || n == 0 || qh == 0 || kvh == 0 || hd == 0 || n > TREE_MAX_NODES || qh % kvh ||
       !cache_type_name(type) || max_positions > 0xFFFFFFFFull || qh > 65535u || hd > KV_MAX_HEAD_DIM)
     return 0;
-  return tree_ws_floats(tree_splits(max_positions, (uint32_t)n, qh, kvh, hd, type), (uint32_t)n, qh, hd) * 4;
+  return tree_ws_floats_upto(max_positions, (uint32_t)n, qh, kvh, hd, type) * 4;
 }
 
 int32_t rf_attention_tree(rf_ctx* ctx, const float* q, uint64_t q_stride, const rf_kv_cache* cache, uint64_t hist_len,
@@ -245,8 +245,8 @@ int32_t rf_attention_tree(rf_ctx* ctx, const float* q, uint64_t q_stride, const 
   a.hist = hist_len; a.n = (uint32_t)n; a.qh = q_heads;
   a.q_vec = (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && q_stride % 4 == 0;
   // with a length word the context may grow to the whole cache under a captured call
-  const uint64_t total = a.cache.length ? a.cache.cap : hist_len + n;
-  a.nsplit = tree_splits(total, a.n, q_heads, a.cache.kvh, a.cache.hd, a.cache.type);
+  a.total = a.cache.length ? a.cache.cap : hist_len + n;
+  a.nsplit = tree_splits(a.total, a.n, q_heads, a.cache.kvh, a.cache.hd, a.cache.type);
   hipStream_t st = pick_stream(ctx, s);
   RF_ON_DEVICE(ctx);
   const uint64_t ws = tree_ws_floats(a.nsplit, a.n, q_heads, a.cache.hd) * 4;

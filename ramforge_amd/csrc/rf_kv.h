@@ -75,16 +75,23 @@ struct TreeArgs {
   uint64_t out_stride;
   KvView cache;
   const uint64_t* mask;  // [n][ceil(n / 64)] or null: token i sees drafts 0..i
-  uint64_t hist;
+  uint64_t hist, total;  // keys before the drafts, and in all (with a length word: at most, nsplit is chosen for it)
   uint32_t n, qh;
   uint32_t nsplit;  // position splits; > 1: records in ws
   uint32_t q_vec;   // q rows are 16-byte aligned
   float* ws;
+  // what a kernel would otherwise work out before its first load (launch_attention_tree)
+  uint32_t group, rows, words;        // query heads and rows of a KV head, words of a mask row
+  uint32_t code_row, scale_row;       // bytes of a position
+  uint64_t scale_base;                // of the scales, from the codes
+  uint32_t tiles, per;                // tiles of 32 positions in all and of a split, without a length word
 };
 // Splits of a call over `total` positions, and the workspace floats they need.
 uint32_t tree_splits(uint64_t total, uint32_t n, uint32_t qh, uint32_t kvh, uint32_t hd, uint32_t type);
 uint64_t tree_ws_floats(uint32_t nsplit, uint32_t n, uint32_t qh, uint32_t hd);
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t st);
+// Workspace floats of every call of up to `total` positions and n tokens.
+uint64_t tree_ws_floats_upto(uint64_t total, uint32_t n, uint32_t qh, uint32_t kvh, uint32_t hd, uint32_t type);
 hipError_t load_module_kv();
 hipError_t load_module_tree();
 

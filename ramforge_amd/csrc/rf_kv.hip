@@ -20,55 +20,91 @@ __device__ __forceinline__ float row8_max(float v) {
   return fmaxf(v, rf_xchg16<4>(v));
 }
 
-// The least float of BITS significant bits (none below 2^-24) that is >= t > 0.
+// The least float of BITS significant bits (none below 2^-24) that is >= t >= 0.
 template <int BITS>
 __device__ __forceinline__ float scale_up(float t) {
   constexpr uint32_t LOW = (1u << (24 - BITS)) - 1u;
   // 2^(BITS - 25) and above: BITS bits of significand are multiples of 2^-24
-  if (t >= (BITS == 3 ? 0x1p-22f : 0x1p-17f)) return __uint_as_float((__float_as_uint(t) + LOW) & ~LOW);
-  return ceilf(t * 0x1p24f) * 0x1p-24f;
+  return t >= (BITS == 3 ? 0x1p-22f : 0x1p-17f) ? __uint_as_float((__float_as_uint(t) + LOW) & ~LOW)
+                                                : ceilf(t * 0x1p24f) * 0x1p-24f;
 }
 
-// The nearest whole number to x / d, ties to even.  x * (1 / d) is off by an
-// ulp or two; the remainder x - q d is exact (q d has at most 15 bits) and
-// says on which side of the half step x lies.
-__device__ __forceinline__ float nearest_code(float x, float d, float inv) {
-  float q = rintf(x * inv);
+// The nearest whole number to x / d, ties to even: the remainder x - q d is
+// exact (q d has at most 15 bits) and says on which side of the half step x
+// lies.
+__device__ __forceinline__ float nearest_code(float x, float d) {
+  x = fminf(fmaxf(x, -8192.f * fabsf(d)), 8192.f * fabsf(d));  // past every clamp; keeps the remainder finite
+  float q = rintf(x / d);
   const float r = fmaf(-q, d, x), h = 0.5f * fabsf(d), a = fabsf(r);
   if (a > h || (a == h && ((int)q & 1))) q += (r > 0.f) == (d > 0.f) ? 1.f : -1.f;
   return q;
 }
 
 // Scale and codes (with their offset) of one lane's four values of a block.
+//
+// A code is the nearest to x / d.  y = x * (1 / d) is off by less than
+// |y| 2^-22 < 4e-5, so its nearest is that of the quotient unless y is that
+// close to a half: then, or where the scale is cut at its largest, the
+// wavefront takes the exact way (nearest_code).  Random values do so once in
+// about 40 wavefronts; with the exact way alone the stores are bound by vector
+// instructions (8191 x 1024 rows into Q4_0: 25.8 us, 3.0 TB/s).
 template <bool Q8>
 __device__ __forceinline__ uint32_t quantise4(const float (&x)[4], uint32_t* scale_bits) {
+  constexpr float LEVELS = Q8 ? 127.f : 8.f, LARGEST = Q8 ? 512.f : 8160.f;
+  constexpr int BITS = Q8 ? 3 : 8;
   float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
   float lo = fmaxf(fmaxf(-x[0], -x[1]), fmaxf(-x[2], -x[3]));
-  bool odd = false;  // an infinity or NaN
-#pragma unroll
-  for (int i = 0; i < 4; ++i) odd |= !(fabsf(x[i]) <= 3.402823466e38f);
+  // an infinity or NaN: 0 * x is NaN
+  float odd = fmaf(0.f, x[0], fmaf(0.f, x[1], fmaf(0.f, x[2], 0.f * x[3]))) == 0.f ? 0.f : 1.f;
   hi = row8_max(hi);
   lo = row8_max(lo);
-  odd = row8_max(odd ? 1.f : 0.f) != 0.f;
-  const float top = fmaxf(hi, lo);
-  constexpr float LEVELS = Q8 ? 127.f : 8.f;
-  float d = scale_up<Q8 ? 3 : 8>(top / LEVELS);
-  // the division may have rounded down to a scale that does not reach the top
-  if (d * LEVELS < top) d = scale_up<Q8 ? 3 : 8>(__uint_as_float(__float_as_uint(d) + 1u));
-  d = fminf(d, Q8 ? 512.f : 8160.f);
-  if (top == 0.f) d = 0.f;
+  odd = row8_max(odd);
+  const float top = odd == 0.f ? fmaxf(hi, lo) : 0.f;
+  float d;
+  if constexpr (Q8) {
+    // from just below top / 127, so that the scale is at most one step low
+    d = scale_up<BITS>(top * 0x1.0204p-7f);
+    if (d * LEVELS < top) d = scale_up<BITS>(__uint_as_float(__float_as_uint(d) + 1u));
+  } else {
+    d = scale_up<BITS>(top * 0.125f);
+    if (d * LEVELS < top) d = 0x1p-24f;  // top / 8 was no float
+  }
+  bool exact = d > LARGEST;
+  d = fminf(d, LARGEST);
   if (!Q8 && hi > lo) d = -d;
-  const float inv = d != 0.f ? 1.f / d : 0.f;
-  uint32_t w = 0;
+  const float inv = d != 0.f ? __builtin_amdgcn_rcpf(d) : 0.f;
+  // the sum's low bits are the nearest whole number (|y| <= 128)
+  constexpr float MAGIC = 12582912.f;
+  float r[4], far = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // 8192 codes are past every clamp; it keeps far values' remainders finite
-    const float xi = odd ? 0.f : fminf(fmaxf(x[i], -8192.f * fabsf(d)), 8192.f * fabsf(d));
-    float q = d != 0.f ? nearest_code(xi, d, inv) : 0.f;
-    q = Q8 ? fminf(fmaxf(q, -127.f), 127.f) + 128.f : fminf(fmaxf(q, -8.f), 7.f) + 8.f;
-    w |= (uint32_t)q << (Q8 ? 8 * i : 4 * i);
+    const float y = x[i] * inv;
+    r[i] = y + MAGIC;
+    far = fmaxf(far, fabsf(y - (r[i] - MAGIC)));
   }
-  *scale_bits = odd ? 0x7E00u : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)d);
+  exact |= far > 0.5f - 5e-5f;
+  if (__any(exact)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float q = d != 0.f ? nearest_code(x[i], d) : 0.f;
+      q = fminf(fmaxf(q, -LEVELS), LEVELS);
+      r[i] = q + MAGIC;
+    }
+  }
+  uint32_t w;
+  if constexpr (Q8) {
+    const uint32_t ab = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x0C0C0400u);
+    const uint32_t cd = __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x04000C0Cu);
+    w = (ab | cd) ^ 0x80808080u;
+    if (odd != 0.f) w = 0x80808080u;
+  } else {
+    uint32_t n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = __float_as_uint(fminf(r[i], MAGIC + 7.f)) + 8u & 15u;
+    w = n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12;
+    if (odd != 0.f) w = 0x8888u;
+  }
+  *scale_bits = odd != 0.f ? 0x7E00u : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)d);
   return w;
 }
 
@@ -123,56 +159,107 @@ __device__ __forceinline__ void get4(const uint8_t* b, uint32_t type, uint64_t c
 
 // ------------------------------------------------------------- store, load
 
-// Threads map to (row, 4 values): a row takes tpr threads, a workgroup holds
-// 256 / tpr rows (or 1024 values of one wide row).  VEC: all rows and widths
-// allow 16-byte accesses; else (F32 / F16 only, or strided rows) by value.
-template <bool LOAD, bool VEC>
+// Where a thread's four values of a row lie.  Threads map to (row, 4 values): a
+// row takes tpr threads, a workgroup holds 256 / tpr rows, or 1024 values of
+// one wide row.
+struct RowMap {
+  uint32_t width, rpw, row, col;
+  bool ok;
+};
+__device__ __forceinline__ RowMap row_map(const KvView& c) {
+  RowMap m;
+  m.width = c.kvh * c.hd;
+  const uint32_t tpr = (m.width + 3u) / 4u, tid = threadIdx.x;
+  m.rpw = tpr < 256u ? 256u / tpr : 1u;
+  m.row = tpr < 256u ? tid / tpr : 0u;
+  m.col = 4u * (tpr < 256u ? tid % tpr : blockIdx.y * 256u + tid);
+  m.ok = m.col < m.width && m.row < m.rpw;
+  return m;
+}
+
+// Rows of 16-byte pieces.  Bound by HBM once the loads are many enough in
+// flight: a thread asks for U rows before it uses the first, with addresses
+// clamped instead of branches (a load in a branch is waited for there).  8191
+// rows of 1024 values into Q4_0, 76 MB: 25.8 us with the exact rounding for
+// every value, 21.4 us without it and one row a thread.
+template <bool LOAD, uint32_t T, int U>
 __global__ __launch_bounds__(256) void kv_rows(KvView c, float* k, uint64_t k_stride, float* v, uint64_t v_stride,
                                                uint64_t first, uint64_t n) {
-  const uint32_t width = c.kvh * c.hd, tpr = (width + 3u) / 4u, rpw = tpr < 256u ? 256u / tpr : 1u;
-  const uint32_t tid = threadIdx.x, r = tpr < 256u ? tid / tpr : 0u;
-  const uint32_t col = 4u * (tpr < 256u ? tid % tpr : blockIdx.y * 256u + tid);
-  float* const x = blockIdx.z ? v : k;
-  const uint64_t stride = blockIdx.z ? v_stride : k_stride, cap_values = c.cap * width;
+  const RowMap m = row_map(c);
+  const uint32_t col = m.ok ? m.col : 0u, lane = threadIdx.x;
+  float* const x = (blockIdx.z ? v : k) + col;
+  const uint64_t stride = blockIdx.z ? v_stride : k_stride, cap_values = c.cap * m.width;
   uint8_t* const b = blockIdx.z ? c.v : c.k;
   const uint64_t base = first + (c.length ? *c.length : 0u);
-  const bool lane_ok = col < width && r < rpw;
-  for (uint64_t i0 = (uint64_t)blockIdx.x * rpw; i0 < n; i0 += (uint64_t)gridDim.x * rpw) {
-    const uint64_t i = i0 + r, row = base + i;
-    const bool ok = lane_ok && i < n && row < c.cap;
-    const uint64_t at = ok ? row * width + col : 0u;
-    float* const xp = x + (ok ? i * stride + col : 0u);
+  for (uint64_t i0 = (uint64_t)blockIdx.x * (m.rpw * U); i0 < n; i0 += (uint64_t)gridDim.x * (m.rpw * U)) {
+    float f[U][4];
+    bool ok[U];
+    uint64_t i[U], at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t want = i0 + u * m.rpw + m.row;
+      i[u] = min(want, n - 1u);
+      ok[u] = m.ok && want < n && base + want < c.cap;
+      at[u] = min(base + i[u], c.cap - 1u) * m.width + col;
+      if constexpr (LOAD) {
+        get4(b, T, cap_values, at[u], f[u]);
+      } else {
+        const float4 t = *reinterpret_cast<const float4*>(x + i[u] * stride);
+        f[u][0] = t.x; f[u][1] = t.y; f[u][2] = t.z; f[u][3] = t.w;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if constexpr (!LOAD) put4(b, T, cap_values, at[u], f[u], lane, ok[u]);
+      else if (ok[u]) *reinterpret_cast<float4*>(x + i[u] * stride) = make_float4(f[u][0], f[u][1], f[u][2], f[u][3]);
+    }
+  }
+}
+
+// Any width, stride and alignment, by value.
+template <bool LOAD>
+__global__ __launch_bounds__(256) void kv_rows_any(KvView c, float* k, uint64_t k_stride, float* v, uint64_t v_stride,
+                                                   uint64_t first, uint64_t n) {
+  const RowMap m = row_map(c);
+  float* const x = blockIdx.z ? v : k;
+  const uint64_t stride = blockIdx.z ? v_stride : k_stride, cap_values = c.cap * m.width;
+  uint8_t* const b = blockIdx.z ? c.v : c.k;
+  const uint64_t base = first + (c.length ? *c.length : 0u);
+  const bool quant = c.type == T_Q8_0 || c.type == T_Q4_0;  // width is then a multiple of 32
+  for (uint64_t i0 = (uint64_t)blockIdx.x * m.rpw; i0 < n; i0 += (uint64_t)gridDim.x * m.rpw) {
+    const uint64_t i = i0 + m.row, row = base + i;
+    const bool ok = m.ok && i < n && row < c.cap;
+    const uint64_t at = ok ? row * m.width + m.col : 0u;
+    const uint32_t ne = ok ? min(4u, m.width - m.col) : 0u;
+    float* const xp = x + (ok ? i * stride + m.col : 0u);
     float f[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (LOAD) {
-      if (!ok) continue;
-      if (c.type == T_Q8_0 || c.type == T_Q4_0 || width % 4u == 0u) {
-        get4(b, c.type, cap_values, at, f);
-      } else {
-        for (uint32_t e = 0; e < min(4u, width - col); ++e)
-          f[e] = c.type == T_F32 ? reinterpret_cast<const float*>(b)[at + e]
-                                 : (float)reinterpret_cast<const _Float16*>(b)[at + e];
-      }
-      if constexpr (VEC) {
-        *reinterpret_cast<float4*>(xp) = make_float4(f[0], f[1], f[2], f[3]);
-      } else {
-        for (uint32_t e = 0; e < min(4u, width - col); ++e) xp[e] = f[e];
-      }
+      if (quant) get4(b, c.type, cap_values, at, f);
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e)
+        if (e < ne)
+          xp[e] = quant ? f[e] : c.type == T_F32 ? reinterpret_cast<const float*>(b)[at + e]
+                                                 : (float)reinterpret_cast<const _Float16*>(b)[at + e];
     } else {
-      if (ok) {
-        if constexpr (VEC) {
-          const float4 t = *reinterpret_cast<const float4*>(xp);
-          f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
-        } else {
-          for (uint32_t e = 0; e < min(4u, width - col); ++e) f[e] = xp[e];
-        }
-      }
-      if (width % 4u == 0u) {
-        put4(b, c.type, cap_values, at, f, tid, ok);
-      } else if (ok) {
-        for (uint32_t e = 0; e < min(4u, width - col); ++e) put1(b, c.type, at + e, f[e]);
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e)
+        if (e < ne) f[e] = xp[e];
+      if (quant) {
+        put4(b, c.type, cap_values, at, f, threadIdx.x, ok);
+      } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+          if (e < ne) put1(b, c.type, at + e, f[e]);
       }
     }
   }
+}
+
+template <bool LOAD, uint32_t T>
+static void launch_rows_vec(bool ahead, dim3 grid, const KvView& c, float* k, uint64_t ks, float* v, uint64_t vs,
+                            uint64_t first, uint64_t n, hipStream_t st) {
+  if (ahead) RF_KLAUNCH((kv_rows<LOAD, T, 4>), grid, dim3(256), 0, st, c, k, ks, v, vs, first, n);
+  else RF_KLAUNCH((kv_rows<LOAD, T, 1>), grid, dim3(256), 0, st, c, k, ks, v, vs, first, n);
 }
 
 template <bool LOAD>
@@ -181,10 +268,21 @@ static hipError_t launch_rows(const KvView& c, float* k, uint64_t ks, float* v, 
   const uint32_t width = c.kvh * c.hd, tpr = (width + 3u) / 4u, rpw = tpr < 256u ? 256u / tpr : 1u;
   const bool vec = width % 4u == 0u && ks % 4u == 0u && vs % 4u == 0u &&
                    ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0u;
-  const uint64_t wgs = (n + rpw - 1) / rpw;
-  const dim3 grid((uint32_t)(wgs < 65536 ? wgs : 65536), (tpr + 255u) / 256u, 2);
-  if (vec) RF_KLAUNCH((kv_rows<LOAD, true>), grid, dim3(256), 0, st, c, k, ks, v, vs, first, n);
-  else RF_KLAUNCH((kv_rows<LOAD, false>), grid, dim3(256), 0, st, c, k, ks, v, vs, first, n);
+  // four rows a thread where that leaves 8 workgroups a CU
+  const uint32_t wide = (tpr + 255u) / 256u;
+  const bool ahead = vec && n * 2 * wide >= (uint64_t)rpw * 4 * 2048;
+  const uint64_t per = (uint64_t)rpw * (ahead ? 4 : 1), wgs = (n + per - 1) / per;
+  const dim3 grid((uint32_t)(wgs < 65536 ? wgs : 65536), wide, 2);
+  if (!vec) {
+    RF_KLAUNCH((kv_rows_any<LOAD>), grid, dim3(256), 0, st, c, k, ks, v, vs, first, n);
+    return hipGetLastError();
+  }
+  switch (c.type) {
+    case T_F32: launch_rows_vec<LOAD, T_F32>(ahead, grid, c, k, ks, v, vs, first, n, st); break;
+    case T_F16: launch_rows_vec<LOAD, T_F16>(ahead, grid, c, k, ks, v, vs, first, n, st); break;
+    case T_Q8_0: launch_rows_vec<LOAD, T_Q8_0>(ahead, grid, c, k, ks, v, vs, first, n, st); break;
+    default: launch_rows_vec<LOAD, T_Q4_0>(ahead, grid, c, k, ks, v, vs, first, n, st);
+  }
   return hipGetLastError();
 }
 
@@ -204,7 +302,7 @@ struct MoveArgs {
   uint8_t *k[KV_MOVE_CACHES], *v[KV_MOVE_CACHES];
   const uint32_t *src, *length;
   uint64_t cap, first, code_row, scale_row, scale_base;  // bytes
-  uint32_t n, code_units, units, slice;                  // units of U bytes in a row: codes, all; per workgroup
+  uint32_t n, code_units, units, slice;                  // units of U bytes in a row: codes, all; log2 of a workgroup's
 };
 
 // A workgroup takes `slice` units of every row of one buffer: all its reads
@@ -215,21 +313,35 @@ __global__ __launch_bounds__(256) void kv_move(MoveArgs a) {
   __shared__ U held[KV_MOVE_MAX];
   const uint32_t cache = blockIdx.y >> 1;
   uint8_t* const b = blockIdx.y & 1u ? a.v[cache] : a.k[cache];
-  const uint32_t u0 = blockIdx.x * a.slice, un = min(a.slice, a.units - u0), items = a.n * un;
-  const uint64_t base = a.length ? *a.length : 0u;
-  const uint64_t first = a.first + base;
+  const uint32_t u0 = blockIdx.x << a.slice, mask = (1u << a.slice) - 1u, items = a.n << a.slice;  // <= KV_MOVE_MAX
+  const uint64_t base = a.length ? *a.length : 0u, first = a.first + base;
   auto addr = [&](uint64_t row, uint32_t u) {
     return u < a.code_units ? b + row * a.code_row + (uint64_t)u * sizeof(U)
                             : b + a.scale_base + row * a.scale_row + (uint64_t)(u - a.code_units) * sizeof(U);
   };
-  for (uint32_t t = threadIdx.x; t < items; t += 256u) {
-    const uint64_t row = base + a.src[t / un];
-    if (row < a.cap) held[t] = *reinterpret_cast<const U*>(addr(row, u0 + t % un));
+  constexpr uint32_t PER = KV_MOVE_MAX / 256u;
+  uint64_t row[PER];
+  bool moves[PER];
+  U x[PER];
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) {
+    const uint32_t t = threadIdx.x + 256u * i;
+    row[i] = t < items ? base + a.src[t >> a.slice] : ~0ull;
   }
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) {
+    const uint32_t t = threadIdx.x + 256u * i, u = u0 + (t & mask);
+    moves[i] = t < items && u < a.units && row[i] < a.cap && first + (t >> a.slice) < a.cap;
+    if (moves[i]) x[i] = *reinterpret_cast<const U*>(addr(row[i], u));
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i)
+    if (moves[i]) held[threadIdx.x + 256u * i] = x[i];
   __syncthreads();
-  for (uint32_t t = threadIdx.x; t < items; t += 256u) {
-    const uint64_t row = first + t / un;
-    if (base + a.src[t / un] < a.cap && row < a.cap) *reinterpret_cast<U*>(addr(row, u0 + t % un)) = held[t];
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) {
+    const uint32_t t = threadIdx.x + 256u * i;
+    if (moves[i]) *reinterpret_cast<U*>(addr(first + (t >> a.slice), u0 + (t & mask))) = held[t];
   }
 }
 
@@ -246,11 +358,11 @@ hipError_t launch_kv_move(const KvView* caches, uint32_t n_caches, const uint32_
   const uint32_t unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
   a.code_units = (uint32_t)(a.code_row / unit);
   a.units = (uint32_t)((a.code_row + a.scale_row) / unit);
-  a.slice = KV_MOVE_MAX / n < a.units ? KV_MOVE_MAX / n : a.units;
+  while ((n << (a.slice + 1)) <= KV_MOVE_MAX && (1u << a.slice) < a.units) ++a.slice;
   for (uint32_t at = 0; at < n_caches; at += KV_MOVE_CACHES) {
     const uint32_t m = n_caches - at < KV_MOVE_CACHES ? n_caches - at : KV_MOVE_CACHES;
     for (uint32_t i = 0; i < m; ++i) { a.k[i] = caches[at + i].k; a.v[i] = caches[at + i].v; }
-    const dim3 grid((a.units + a.slice - 1) / a.slice, 2 * m);
+    const dim3 grid((a.units + (1u << a.slice) - 1) >> a.slice, 2 * m);
     if (unit == 16) RF_KLAUNCH(kv_move<uint4>, grid, dim3(256), 0, st, a);
     else if (unit == 4) RF_KLAUNCH(kv_move<uint32_t>, grid, dim3(256), 0, st, a);
     else RF_KLAUNCH(kv_move<uint16_t>, grid, dim3(256), 0, st, a);

@@ -354,7 +354,7 @@ template <int HD> struct TreeTile<T_F32, HD> {
   static __device__ __forceinline__ constexpr int order(int i) { return i; }
 };
 
-constexpr float TREE_FLOOR = -1e30f;  // reference of a row that has seen nothing
+constexpr float TREE_FLOOR = -3e38f;  // reference of a row that has seen nothing
 // A row's reference is set 2^12 below its largest score and moves once a weight
 // would pass 2^15: weights stay inside f16, and as far as can be above its
 // subnormals, which a weight 2^-26 of the largest meets.
@@ -366,12 +366,19 @@ __device__ __forceinline__ void tree_lds_order() {  // within a wavefront
   __builtin_amdgcn_wave_barrier();
 }
 
-// Two f16 pieces of x and y: the nearest halves, and the nearest of what they leave.
-__device__ __forceinline__ void tree_pieces(float x, float y, uint32_t& hi, uint32_t& lo) {
+// Two f16 pieces of x and y: the nearest halves, and the nearest of what they
+// leave.  minus: -1 that the compiler cannot see through, so that the rest is
+// one mixed-precision fma each and no conversion back.
+__device__ __forceinline__ float tree_minus() {
+  float m = -1.f;
+  asm volatile("" : "+v"(m));
+  return m;
+}
+__device__ __forceinline__ void tree_pieces(float x, float y, float minus, uint32_t& hi, uint32_t& lo) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const half2_t h = __builtin_convertvector((f32x2{x, y}), half2_t);
   hi = __builtin_bit_cast(uint32_t, h);
-  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{fmaf((float)h[0], -1.f, x), fmaf((float)h[1], -1.f, y)}), half2_t));
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{fmaf((float)h[0], minus, x), fmaf((float)h[1], minus, y)}), half2_t));
 }
 
 // Shared memory of a workgroup: Q's operands (all its wavefronts have the same
@@ -405,6 +412,7 @@ __device__ __forceinline__ void tree_get_q(float (&x)[HD / 4], const float* qp, 
 // that takes the scores to powers of two is returned.
 template <uint32_t T, int HD, typename Put>
 __device__ __forceinline__ float tree_split_q(const float (&x)[HD / 4], Put put) {
+  const float minus = tree_minus();
   float scale = 1.44269504088896340736f / sqrtf((float)HD), top = 0.f, up = 1.f;
 #pragma unroll
   for (int i = 0; i < HD / 4; ++i) top = fmaxf(top, fabsf(x[i]));
@@ -422,7 +430,7 @@ __device__ __forceinline__ float tree_split_q(const float (&x)[HD / 4], Put put)
     for (int i = 0; i < 4; ++i) {
       using Tile = TreeTile<T, HD>;
       uint32_t h, r;
-      tree_pieces(x[8 * s + Tile::order(2 * i)] * up, x[8 * s + Tile::order(2 * i + 1)] * up, h, r);
+      tree_pieces(x[8 * s + Tile::order(2 * i)] * up, x[8 * s + Tile::order(2 * i + 1)] * up, minus, h, r);
       hi[i] = h;
       lo[i] = r;
     }
@@ -507,22 +515,39 @@ __device__ __forceinline__ void tree_soften(f32x4 (&s)[2], uint32_t see, float s
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j / 4][j % 4] = see >> j & 1u ? s[j / 4][j % 4] : -INFINITY;
   }
-  float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                    fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+  // exponents against the reference, and the largest of them
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    p[j] = fmaf(s[j / 4][j % 4], scale, -ref);
+    top = fmaxf(top, p[j]);
+  }
   // The reference stays until a weight would pass 2^15: few tiles rescale.
-  if (__any(fmaf(top, scale, -ref) > TREE_MOST)) {
+  if (__any(top > TREE_MOST)) {
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float now = fmaxf(ref, fmaf(top, scale, -TREE_BELOW)), al = exp2f(ref - now);
+    // against the old reference; a row that has seen nothing starts from its scores
+    const bool first = ref == TREE_FLOOR;
+    float best = -INFINITY;
+    if (first) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) best = fmaxf(best, s[j / 4][j % 4]);
+    }
+    best = fmaxf(best, __shfl_xor(best, 16));
+    best = fmaxf(best, __shfl_xor(best, 32));
+    const float now = first ? fmaxf(ref, fmaf(best, scale, -TREE_BELOW)) : ref + fmaxf(0.f, top - TREE_BELOW);
+    const float al = first ? 0.f : __builtin_amdgcn_exp2f(ref - now);
     ref = now;
     l *= al;
 #pragma unroll
     for (int d = 0; d < TreeDims<HD>::TILES; ++d)
 #pragma unroll
       for (int v = 0; v < 4; ++v) o[d][v] *= al;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = fmaf(s[j / 4][j % 4], scale, -ref);
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], scale, -ref));
+  for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(p[j]);
   l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 }
 
@@ -587,7 +612,7 @@ constexpr int tree_waves_per_simd(uint32_t type, int hd, int m) {
   return (type == T_F32 && hd * m >= 256) || (hd == 256 && (type == T_F16 || type == T_Q8_0)) || hd * m > 256 ? 1 : 2;
 }
 template <uint32_t T, int HD, int M>
-__global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) void tree_mfma(TreeArgs a, uint32_t row_blocks) {
+__global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) void tree_mfma(TreeArgs a) {
   using D = TreeDims<HD>;
   using Tile = TreeTile<T, HD>;
   using S = TreeShared<T, HD, M>;
@@ -595,8 +620,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
   __shared__ S sh;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: the tiles' descriptors are scalars
-  const uint32_t split = blockIdx.x, head = blockIdx.y / row_blocks, row0 = blockIdx.y % row_blocks * (M * 16u);
-  const uint32_t G = a.qh / a.cache.kvh, rows = a.n * G, words = (a.n + 63u) / 64u;
+  const uint32_t split = blockIdx.x, head = blockIdx.z, row0 = blockIdx.y * (M * 16u);
+  const uint32_t G = a.group, rows = a.rows, words = a.words;
 
   // this lane's Q: wavefront w has row tiles w, w + 4, ..; requested before the cache's rows
   float x[HD / 4];
@@ -609,13 +634,16 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
   if (wave < (uint32_t)M) ask_q((int)wave);
   __builtin_amdgcn_sched_barrier(0);
 
-  uint64_t hist, total;
-  tree_range(a, hist, total);
-  const uint32_t tiles = (uint32_t)((total + TREE_KEYS - 1u) / TREE_KEYS), per = (tiles + a.nsplit - 1u) / a.nsplit;
+  uint64_t hist = a.hist, total = a.total;
+  uint32_t tiles = a.tiles, per = a.per;
+  if (a.cache.length) {
+    tree_range(a, hist, total);
+    tiles = (uint32_t)((total + TREE_KEYS - 1u) / TREE_KEYS);
+    per = (tiles + a.nsplit - 1u) / a.nsplit;
+  }
   const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
-  const uint32_t width = a.cache.kvh * HD;
-  const uint32_t row = T == T_F32 ? width * 4u : T == T_F16 ? width * 2u : T == T_Q8_0 ? width : width / 2u, srow = width / 16u;
-  const uint64_t sbase = a.cache.cap * (uint64_t)row;
+  const uint32_t row = a.code_row, srow = a.scale_row;
+  const uint64_t sbase = a.scale_base;
   Tile cur;
   // Bounded descriptors: rows behind the last read as zeros, and nothing is
   // read for a tile behind the last.  The loads are in no branch and in this
@@ -645,6 +673,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
   uint32_t tok[M];
   float scale[M], ref[M], l[M];
   f32x4 o[M][D::TILES];
+  const float minus = tree_minus();
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     tok[m] = min(row0 + 16u * m + c, rows - 1u) / G;
@@ -719,7 +748,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t h, r;
-          tree_pieces(p[m][2 * j], p[m][2 * j + 1], h, r);
+          tree_pieces(p[m][2 * j], p[m][2 * j + 1], minus, h, r);
           ph[m][j] = h;
           pl[m][j] = r;
         }
@@ -751,7 +780,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
       float top = TREE_FLOOR;
 #pragma unroll
       for (uint32_t w = 0; w < TREE_WAVES; ++w) top = fmaxf(top, sh.m[w][16 * m + c]);
-      const float al = exp2f(ref[m] - top);
+      const float al = __builtin_amdgcn_exp2f(ref[m] - top);
 #pragma unroll
       for (int d = 0; d < D::TILES; ++d)
 #pragma unroll
@@ -764,10 +793,12 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
         const uint32_t rr = e / (S::CH / 4u), dd = e % (S::CH / 4u) * 4u, d = part * S::CH + dd, r = row0 + 16u * m + rr;
         if (r >= rows) continue;
         float best = TREE_FLOOR, sum = 0.f;
+        if (a.nsplit == 1 || d == 0) {
 #pragma unroll
-        for (uint32_t w = 0; w < TREE_WAVES; ++w) best = fmaxf(best, sh.m[w][16 * m + rr]);
+          for (uint32_t w = 0; w < TREE_WAVES; ++w) best = fmaxf(best, sh.m[w][16 * m + rr]);
 #pragma unroll
-        for (uint32_t w = 0; w < TREE_WAVES; ++w) sum += sh.l[w][16 * m + rr] * exp2f(sh.m[w][16 * m + rr] - best);
+          for (uint32_t w = 0; w < TREE_WAVES; ++w) sum += sh.l[w][16 * m + rr] * __builtin_amdgcn_exp2f(sh.m[w][16 * m + rr] - best);
+        }
         float4 y = *reinterpret_cast<const float4*>(&sh.sum[0][rr * S::OP + dd]);
 #pragma unroll
         for (uint32_t w = 1; w < TREE_WAVES; ++w) {
@@ -848,23 +879,25 @@ template <int HD> struct TreeRowsShared {
 };
 
 template <uint32_t T, int HD, int M>
-__global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a, uint32_t row_blocks) {
+__global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a) {
   using D = TreeDims<HD>;
   using Tile = TreeTile<T, HD>;
   using Part = TreePart<T, HD>;
   __shared__ TreeRowsShared<HD> sh;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t split = blockIdx.x, head = blockIdx.y / row_blocks;
-  const uint32_t row0 = (blockIdx.y % row_blocks * TREE_WAVES + wave) * (M * 16u);
-  const uint32_t G = a.qh / a.cache.kvh, rows = a.n * G, words = (a.n + 63u) / 64u;
-  uint64_t hist, total;
-  tree_range(a, hist, total);
-  const uint32_t tiles = (uint32_t)((total + TREE_KEYS - 1u) / TREE_KEYS), per = (tiles + a.nsplit - 1u) / a.nsplit;
+  const uint32_t split = blockIdx.x, head = blockIdx.z, row0 = (blockIdx.y * TREE_WAVES + wave) * (M * 16u);
+  const uint32_t G = a.group, rows = a.rows, words = a.words;
+  uint64_t hist = a.hist, total = a.total;
+  uint32_t tiles = a.tiles, per = a.per;
+  if (a.cache.length) {
+    tree_range(a, hist, total);
+    tiles = (uint32_t)((total + TREE_KEYS - 1u) / TREE_KEYS);
+    per = (tiles + a.nsplit - 1u) / a.nsplit;
+  }
   const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
-  const uint32_t width = a.cache.kvh * HD;
-  const uint32_t row = T == T_F16 ? width * 2u : T == T_Q8_0 ? width : width / 2u, srow = width / 16u;
-  const uint64_t sbase = a.cache.cap * (uint64_t)row;
+  const uint32_t row = a.code_row, srow = a.scale_row;
+  const uint64_t sbase = a.scale_base;
   Part part;
   auto fetch = [&](uint32_t tile) {  // as in tree_mfma: in no branch
     const uint64_t p = (uint64_t)tile * TREE_KEYS;
@@ -890,6 +923,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a, uint
   uint32_t tok[M];
   float scale[M], ref[M], l[M];
   f32x4 o[M][D::TILES];
+  const float minus = tree_minus();
   float x[M][HD / 4];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
@@ -941,7 +975,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a, uint
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t h, r;
-        tree_pieces(p[m][2 * j], p[m][2 * j + 1], h, r);
+        tree_pieces(p[m][2 * j], p[m][2 * j + 1], minus, h, r);
         ph[m][j] = h;
         pl[m][j] = r;
       }
@@ -1027,7 +1061,7 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
     for (uint32_t s = part; s < a.nsplit; s += JOIN) {
       const float* const at = rec + s * step;
       const float4 z = *reinterpret_cast<const float4*>(at + d);
-      const float m = at[HD], now = fmaxf(top, m), al = exp2f(top - now), w = exp2f(m - now);
+      const float m = at[HD], now = fmaxf(top, m), al = __builtin_amdgcn_exp2f(top - now), w = __builtin_amdgcn_exp2f(m - now);
       top = now;
       sum = fmaf(sum, al, at[HD + 1] * w);
       o[0] = fmaf(o[0], al, z.x * w); o[1] = fmaf(o[1], al, z.y * w);
@@ -1043,7 +1077,7 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
   for (uint32_t p = 0; p < JOIN; ++p) top = fmaxf(top, y[p][HD]);
 #pragma unroll
   for (uint32_t p = 0; p < JOIN; ++p) {
-    const float w = exp2f(y[p][HD] - top);
+    const float w = __builtin_amdgcn_exp2f(y[p][HD] - top);
     const float4 z = *reinterpret_cast<const float4*>(&y[p][d]);
     sum = fmaf(y[p][HD + 1], w, sum);
     o[0] = fmaf(z.x, w, o[0]); o[1] = fmaf(z.y, w, o[1]); o[2] = fmaf(z.z, w, o[2]); o[3] = fmaf(z.w, w, o[3]);
@@ -1058,56 +1092,87 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
 
 static bool tree_on_matrix_cores(uint32_t hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
-// The kernel of a shape: few rows go to tree_mfma, whose wavefronts split the
-// positions (tiles: row tiles of each), more to tree_rows, whose wavefronts
-// split the rows.
+// The kernel of a shape.  tree_mfma, whose wavefronts split the positions, has
+// few records to join; tree_rows, whose wavefronts split the rows, decodes less.
+// The first is ahead until every CU has 256 pairs of a row tile and a tile of
+// positions (Q8_0, 8 KV heads of 128, us in the first and the second: 64 rows
+// over 8192 positions 18.9 and 27.8, 256 over 8192 36 and 51, 64 over 64000 61
+// and 61, 256 over 32000 102 and 92, 1024 over 8256 136 and 97).  An f32 cache
+// has nothing to decode and stays with it.
+//
+// Row tiles of a wavefront in the first: two where that leaves a workgroup for
+// every CU, one otherwise (37 tokens over 637 f32 positions: 13.2 us with one,
+// 17.8 with two).
 struct TreePlan {
   bool rows_apart;
   uint32_t tiles, block_rows;  // row tiles of a wavefront, rows of a workgroup
 };
-static TreePlan tree_plan(uint64_t rows, uint32_t hd, uint32_t type) {
-  TreePlan p{rows > 32 && type != T_F32, 1, 16};
+constexpr uint32_t TREE_CUS = 256, TREE_LEAST = 4;  // tiles of a split at least
+static TreePlan tree_plan(uint64_t rows, uint32_t kvh, uint64_t total, uint32_t hd, uint32_t type) {
+  const uint64_t tiles = (total + TREE_KEYS - 1) / TREE_KEYS, work = tiles * kvh * ((rows + 15) / 16);
+  TreePlan p{type != T_F32 && rows > 32 && work > 256 * TREE_CUS, 1, 16};
   if (p.rows_apart) {
     p.tiles = rows > 64 && hd != 256 ? 2 : 1;
     p.block_rows = 16 * TREE_WAVES * p.tiles;
   } else {
-    p.tiles = rows > 16 && hd != 256 ? 2 : 1;
+    const uint64_t splits = (tiles + TREE_LEAST - 1) / TREE_LEAST;
+    p.tiles = rows > 16 && hd != 256 && kvh * ((rows + 15) / 16) * splits > TREE_CUS ? 2 : 1;
     p.block_rows = 16 * p.tiles;
   }
   return p;
 }
 
+// Splits for at most one workgroup a CU (tree_mfma, whose records grow with the
+// splits: 64 rows over 8192 positions 18.9 us, 23.1 with two a CU) or two
+// (tree_rows: 97 us against 109 with one at 1024 rows over 8256).  At most: one
+// workgroup too many is a second round for all (80 rows over 8192 positions
+// 21.7 us with 240 workgroups, 26.8 with 264).
 uint32_t tree_splits(uint64_t total, uint32_t n, uint32_t qh, uint32_t kvh, uint32_t hd, uint32_t type) {
   if (!tree_on_matrix_cores(hd)) return 1;
   const uint64_t rows = (uint64_t)n * (qh / kvh);
-  const TreePlan p = tree_plan(rows, hd, type);
+  const TreePlan p = tree_plan(rows, kvh, total, hd, type);
   const uint64_t units = kvh * ((rows + p.block_rows - 1) / p.block_rows), tiles = (total + TREE_KEYS - 1) / TREE_KEYS;
-  const uint64_t want = (512 + units - 1) / units, least = p.rows_apart ? 4 : TREE_WAVES;  // tiles of a split
-  const uint64_t most = (tiles + least - 1) / least, s = want < most ? want : most;
+  const uint64_t want = (p.rows_apart ? 2 : 1) * TREE_CUS / units;
+  const uint64_t most = (tiles + TREE_LEAST - 1) / TREE_LEAST, s = want < most ? want : most;
   return (uint32_t)(s ? s : 1);
 }
 uint64_t tree_ws_floats(uint32_t nsplit, uint32_t n, uint32_t qh, uint32_t hd) {
   return nsplit > 1 ? (uint64_t)nsplit * n * qh * (hd + 4) : 0;
 }
 
+// A longer context or more tokens may go another way: the most over the ways
+// and over every smaller n (fewer rows, more splits).
+uint64_t tree_ws_floats_upto(uint64_t total, uint32_t n, uint32_t qh, uint32_t kvh, uint32_t hd, uint32_t type) {
+  if (!tree_on_matrix_cores(hd)) return 0;
+  uint64_t most = 0;
+  const uint64_t tiles = (total + TREE_KEYS - 1) / TREE_KEYS, cut = (tiles + TREE_LEAST - 1) / TREE_LEAST;
+  for (uint32_t m = 1; m <= n; ++m) {
+    const uint64_t rows = (uint64_t)m * (qh / kvh);
+    for (uint32_t block : {16u, 32u, 64u, 128u}) {  // rows of a workgroup; two a CU from 64
+      const uint64_t units = kvh * ((rows + block - 1) / block), want = (block < 64 ? 1 : 2) * TREE_CUS / units;
+      const uint64_t s = want < cut ? want : cut, need = tree_ws_floats((uint32_t)s, m, qh, hd);
+      most = need > most ? need : most;
+    }
+  }
+  return most;
+}
+
 template <uint32_t T, int HD>
 static void launch_tree(const TreeArgs& a, hipStream_t st) {
-  const uint64_t rows = (uint64_t)a.n * (a.qh / a.cache.kvh);
-  const TreePlan p = tree_plan(rows, HD, T);
-  const uint32_t blocks = (uint32_t)((rows + p.block_rows - 1) / p.block_rows);
-  const dim3 grid(a.nsplit, a.cache.kvh * blocks), wg(64 * TREE_WAVES);
+  const TreePlan p = tree_plan(a.rows, a.cache.kvh, a.total, HD, T);
+  const dim3 grid(a.nsplit, (a.rows + p.block_rows - 1) / p.block_rows, a.cache.kvh), wg(64 * TREE_WAVES);
   if (p.rows_apart) {
     if constexpr (T != T_F32) {
       if constexpr (HD <= 128) {
-        if (p.tiles == 2) RF_KLAUNCH((tree_rows<T, HD, 2>), grid, wg, 0, st, a, blocks);
+        if (p.tiles == 2) RF_KLAUNCH((tree_rows<T, HD, 2>), grid, wg, 0, st, a);
       }
-      if (p.tiles == 1) RF_KLAUNCH((tree_rows<T, HD, 1>), grid, wg, 0, st, a, blocks);
+      if (p.tiles == 1) RF_KLAUNCH((tree_rows<T, HD, 1>), grid, wg, 0, st, a);
     }
   } else {
     if constexpr (HD <= 128) {
-      if (p.tiles == 2) RF_KLAUNCH((tree_mfma<T, HD, 2>), grid, wg, 0, st, a, blocks);
+      if (p.tiles == 2) RF_KLAUNCH((tree_mfma<T, HD, 2>), grid, wg, 0, st, a);
     }
-    if (p.tiles == 1) RF_KLAUNCH((tree_mfma<T, HD, 1>), grid, wg, 0, st, a, blocks);
+    if (p.tiles == 1) RF_KLAUNCH((tree_mfma<T, HD, 1>), grid, wg, 0, st, a);
   }
   if (a.nsplit > 1) RF_KLAUNCH(tree_join<HD>, dim3(a.n * a.qh), dim3(256), 0, st, a);
 }
@@ -1122,16 +1187,26 @@ static void launch_tree_type(const TreeArgs& a, hipStream_t st) {
   }
 }
 
-hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t st) {
+hipError_t launch_attention_tree(const TreeArgs& args, hipStream_t st) {
+  TreeArgs a = args;
+  const uint64_t width = (uint64_t)a.cache.kvh * a.cache.hd;
+  a.group = a.qh / a.cache.kvh;
+  a.rows = a.n * a.group;
+  a.words = (a.n + 63u) / 64u;
+  a.code_row = (uint32_t)kv_code_bytes(a.cache.type, width);
+  a.scale_row = (uint32_t)(kv_row_bytes(a.cache.type, width) - a.code_row);
+  a.scale_base = a.cache.cap * a.code_row;
+  a.tiles = (uint32_t)((a.total + TREE_KEYS - 1) / TREE_KEYS);
+  a.per = (a.tiles + a.nsplit - 1) / a.nsplit;
   if (!tree_on_matrix_cores(a.cache.hd)) {
     RF_KLAUNCH(tree_plain, dim3(a.n, a.qh), dim3(256), 0, st, a);
-  } else {
-    switch (a.cache.type) {
-      case T_F32: launch_tree_type<T_F32>(a, st); break;
-      case T_F16: launch_tree_type<T_F16>(a, st); break;
-      case T_Q8_0: launch_tree_type<T_Q8_0>(a, st); break;
-      default: launch_tree_type<T_Q4_0>(a, st);
-    }
+    return hipGetLastError();
+  }
+  switch (a.cache.type) {
+    case T_F32: launch_tree_type<T_F32>(a, st); break;
+    case T_F16: launch_tree_type<T_F16>(a, st); break;
+    case T_Q8_0: launch_tree_type<T_Q8_0>(a, st); break;
+    default: launch_tree_type<T_Q4_0>(a, st);
   }
   return hipGetLastError();
 }
