@@ -382,14 +382,26 @@ __device__ __forceinline__ void tree_pieces(float x, float y, float minus, uint3
 }
 
 // Shared memory of a workgroup: Q's operands (all its wavefronts have the same
-// rows), and rows of sums, where the wavefronts join and odd values are added.
+// rows) and where odd values are added, and, once the positions are done, the
+// rows of sums in their place.
+constexpr uint32_t TREE_ODD = 36;
+// Wavefronts of a workgroup of tree_mfma: eight (two a SIMD, one decoding under
+// the other's matrix instructions) where two row tiles keep a CU to itself, four
+// where workgroups are many and small (128 rows over 8192 positions 25.4 us with
+// four, 22.7 with eight; one token over 2048 9.8 and 10.2).
+constexpr int tree_wide(uint32_t type, int hd, int m) { return m == 2 && !(type == T_F32 && hd == 128) ? 8 : 4; }
 template <uint32_t T, int HD, int M> struct TreeShared {
-  static constexpr uint32_t CH = HD < 128 ? HD : 128, PARTS = HD / CH, OP = CH + 4;  // dims of a part of an output row
-  static constexpr uint32_t QW = T == T_F32 ? HD / 16 : HD / 16;  // 16-byte words of a lane's Q
-  u32x4 q[M][QW][64];
+  static constexpr int W = tree_wide(T, HD, M);
+  static constexpr uint32_t OP = HD + 4;  // floats of a row of sums
+  union {
+    struct {
+      u32x4 q[M][HD / 16][64];
+      float odd[W][16 * TREE_ODD];
+    };
+    float sum[W][M * 16 * OP];
+  };
   float scale[M][16];
-  float sum[TREE_WAVES][16 * OP];
-  float m[TREE_WAVES][M * 16], l[TREE_WAVES][M * 16];
+  float m[W][M * 16], l[W][M * 16];
 };
 
 // A lane's HD / 4 values of a row of q.
@@ -464,7 +476,6 @@ __device__ __forceinline__ void tree_put_q(TreeShared<T, HD, M>& sh, int m, floa
 // added, by value, to the rows that do.  Rare, so plain and slow; the sums go
 // through 16 x TREE_ODD floats of LDS, 32 dims at a time, so that no register
 // array is indexed.
-constexpr uint32_t TREE_ODD = 36;
 template <int HD, int M>
 __device__ __forceinline__ void tree_odd_rows(const TreeArgs& a, const float (&p)[M][8], const uint32_t (&see)[M],
                                               uint64_t p0, uint64_t total, uint32_t head, uint32_t c, uint32_t g,
@@ -612,11 +623,12 @@ constexpr int tree_waves_per_simd(uint32_t type, int hd, int m) {
   return (type == T_F32 && hd * m >= 256) || (hd == 256 && (type == T_F16 || type == T_Q8_0)) || hd * m > 256 ? 1 : 2;
 }
 template <uint32_t T, int HD, int M>
-__global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) void tree_mfma(TreeArgs a) {
+__global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 ? 1 : tree_waves_per_simd(T, HD, M)) void tree_mfma(TreeArgs a) {
   using D = TreeDims<HD>;
   using Tile = TreeTile<T, HD>;
   using S = TreeShared<T, HD, M>;
   constexpr bool F32 = T == T_F32;
+  constexpr uint32_t W = S::W;
   __shared__ S sh;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: the tiles' descriptors are scalars
@@ -630,7 +642,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
     const float* const qp = a.q + (uint64_t)i * a.q_stride + ((uint64_t)head * G + (r - i * G)) * HD + g * (HD / 4);
     tree_get_q<HD>(x, qp, a.q_vec);
   };
-  static_assert(M <= (int)TREE_WAVES, "a row tile per wavefront");
+  static_assert(M <= (int)W, "a row tile per wavefront");
   if (wave < (uint32_t)M) ask_q((int)wave);
   __builtin_amdgcn_sched_barrier(0);
 
@@ -719,7 +731,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    fetch_k(tile + TREE_WAVES);  // the old words are spent
+    fetch_k(tile + W);  // the old words are spent
     float p[M][8];
     uint32_t see[M];
 #pragma unroll
@@ -755,14 +767,16 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
       tree_tiles<T, HD, M, DRAFTS, 0>(cur, ph, pl, odd, o);
     }
     __builtin_amdgcn_sched_barrier(0);
-    fetch_v(tile + TREE_WAVES);
-    if (DRAFTS && __any(odd)) tree_odd_rows<HD, M>(a, p, see, p0, total, head, c, g, sh.sum[wave], o);
+    fetch_v(tile + W);
+    if (DRAFTS && __any(odd)) tree_odd_rows<HD, M>(a, p, see, p0, total, head, c, g, sh.odd[wave], o);
   };
   // the drafts come last
-  for (; tile < t1 && (uint64_t)tile * TREE_KEYS + TREE_KEYS <= hist; tile += TREE_WAVES) step(std::false_type());
-  for (; tile < t1; tile += TREE_WAVES) step(std::true_type());
+  for (; tile < t1 && (uint64_t)tile * TREE_KEYS + TREE_KEYS <= hist; tile += W) step(std::false_type());
+  for (; tile < t1; tile += W) step(std::true_type());
 
-  // join the wavefronts, a row tile (and 128 dims) at a time
+  // Join the wavefronts: all their sums in LDS (in Q's place, so once all are
+  // done with it), and what a sum weighs is worked out where it is added.
+  __syncthreads();
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     l[m] += __shfl_xor(l[m], 16);
@@ -771,51 +785,38 @@ __global__ __launch_bounds__(64 * TREE_WAVES, tree_waves_per_simd(T, HD, M)) voi
       sh.m[wave][16 * m + c] = ref[m];
       sh.l[wave][16 * m + c] = l[m];
     }
+#pragma unroll
+    for (int d = 0; d < D::TILES; ++d)
+#pragma unroll
+      for (uint32_t v = 0; v < 4; ++v) sh.sum[wave][(16 * m + c) * S::OP + D::dim(d, 4u * g + v)] = o[m][d][v];
   }
+  __syncthreads();
 #pragma unroll
-  for (int m = 0; m < M; ++m) {
+  for (uint32_t e0 = 0; e0 < M * 16u * HD / 4u; e0 += 64u * W) {
+    const uint32_t e = e0 + tid, rr = e / (HD / 4u), d = e % (HD / 4u) * 4u, r = row0 + rr;
+    if (e >= M * 16u * HD / 4u || r >= rows) continue;
+    float w[W], best = TREE_FLOOR, sum = 0.f;
 #pragma unroll
-    for (uint32_t part = 0; part < S::PARTS; ++part) {
-      __syncthreads();
-      float top = TREE_FLOOR;
+    for (uint32_t k = 0; k < W; ++k) best = fmaxf(best, w[k] = sh.m[k][rr]);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (uint32_t w = 0; w < TREE_WAVES; ++w) top = fmaxf(top, sh.m[w][16 * m + c]);
-      const float al = __builtin_amdgcn_exp2f(ref[m] - top);
+    for (uint32_t k = 0; k < W; ++k) {
+      w[k] = __builtin_amdgcn_exp2f(w[k] - best);
+      sum = fmaf(sh.l[k][rr], w[k], sum);
+      const f32x4 z = *reinterpret_cast<const f32x4*>(&sh.sum[k][rr * S::OP + d]);
 #pragma unroll
-      for (int d = 0; d < D::TILES; ++d)
+      for (int i = 0; i < 4; ++i) y[i] = fmaf(z[i], w[k], y[i]);
+    }
+    const uint32_t i = r / G, h = head * G + (r - i * G);
+    if (a.nsplit == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      float* const out = a.out + (uint64_t)i * a.out_stride + (uint64_t)h * HD + d;
 #pragma unroll
-        for (uint32_t v = 0; v < 4; ++v) {
-          const uint32_t dim = D::dim(d, 4u * g + v);
-          if (S::PARTS == 1 || dim / S::CH == part) sh.sum[wave][c * S::OP + dim % S::CH] = o[m][d][v] * al;
-        }
-      __syncthreads();
-      for (uint32_t e = tid; e < 16u * S::CH / 4u; e += 64u * TREE_WAVES) {
-        const uint32_t rr = e / (S::CH / 4u), dd = e % (S::CH / 4u) * 4u, d = part * S::CH + dd, r = row0 + 16u * m + rr;
-        if (r >= rows) continue;
-        float best = TREE_FLOOR, sum = 0.f;
-        if (a.nsplit == 1 || d == 0) {
-#pragma unroll
-          for (uint32_t w = 0; w < TREE_WAVES; ++w) best = fmaxf(best, sh.m[w][16 * m + rr]);
-#pragma unroll
-          for (uint32_t w = 0; w < TREE_WAVES; ++w) sum += sh.l[w][16 * m + rr] * __builtin_amdgcn_exp2f(sh.m[w][16 * m + rr] - best);
-        }
-        float4 y = *reinterpret_cast<const float4*>(&sh.sum[0][rr * S::OP + dd]);
-#pragma unroll
-        for (uint32_t w = 1; w < TREE_WAVES; ++w) {
-          const float4 z = *reinterpret_cast<const float4*>(&sh.sum[w][rr * S::OP + dd]);
-          y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-        }
-        const uint32_t i = r / G, h = head * G + r % G;
-        if (a.nsplit == 1) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          float* const out = a.out + (uint64_t)i * a.out_stride + (uint64_t)h * HD + d;
-          out[0] = y.x * inv; out[1] = y.y * inv; out[2] = y.z * inv; out[3] = y.w * inv;
-        } else {
-          float* const rec = a.ws + (((uint64_t)split * a.n + i) * a.qh + h) * (HD + 4);
-          *reinterpret_cast<float4*>(rec + d) = y;
-          if (d == 0) { rec[HD] = best; rec[HD + 1] = sum; }
-        }
-      }
+      for (int k = 0; k < 4; ++k) out[k] = y[k] * inv;
+    } else {
+      float* const rec = a.ws + (((uint64_t)split * a.n + i) * a.qh + h) * (HD + 4);
+      *reinterpret_cast<f32x4*>(rec + d) = y;
+      if (d == 0) { rec[HD] = best; rec[HD + 1] = sum; }
     }
   }
 }
@@ -1093,12 +1094,13 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
 static bool tree_on_matrix_cores(uint32_t hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
 // The kernel of a shape.  tree_mfma, whose wavefronts split the positions, has
-// few records to join; tree_rows, whose wavefronts split the rows, decodes less.
-// The first is ahead until every CU has 256 pairs of a row tile and a tile of
-// positions (Q8_0, 8 KV heads of 128, us in the first and the second: 64 rows
-// over 8192 positions 18.9 and 27.8, 256 over 8192 36 and 51, 64 over 64000 61
-// and 61, 256 over 32000 102 and 92, 1024 over 8256 136 and 97).  An f32 cache
-// has nothing to decode and stays with it.
+// few records to join; tree_rows, whose wavefronts split the rows, decodes less
+// and reads the cache fewer times.  The first is ahead until every CU has 5 hd
+// pairs of a row tile and a tile of positions (us in the first and the second,
+// 8 KV heads of 128: 64 rows over 8192 Q8_0 positions 18.7 and 27.8, 256 over
+// 8192 31.5 and 49.4, 1024 over 8256 86 and 94, 64 over 131072 Q4_0 positions
+// 92 and 96, 512 over 32128 163 and 143; 2 of 64, 1400 rows over 16200 F16
+// positions 52 and 45).  An f32 cache has nothing to decode and stays with it.
 //
 // Row tiles of a wavefront in the first: two where that leaves a workgroup for
 // every CU, one otherwise (37 tokens over 637 f32 positions: 13.2 us with one,
@@ -1110,7 +1112,7 @@ struct TreePlan {
 constexpr uint32_t TREE_CUS = 256, TREE_LEAST = 4;  // tiles of a split at least
 static TreePlan tree_plan(uint64_t rows, uint32_t kvh, uint64_t total, uint32_t hd, uint32_t type) {
   const uint64_t tiles = (total + TREE_KEYS - 1) / TREE_KEYS, work = tiles * kvh * ((rows + 15) / 16);
-  TreePlan p{type != T_F32 && rows > 32 && work > 256 * TREE_CUS, 1, 16};
+  TreePlan p{type != T_F32 && rows > 32 && work > 5ull * hd * TREE_CUS, 1, 16};
   if (p.rows_apart) {
     p.tiles = rows > 64 && hd != 256 ? 2 : 1;
     p.block_rows = 16 * TREE_WAVES * p.tiles;
@@ -1123,7 +1125,7 @@ static TreePlan tree_plan(uint64_t rows, uint32_t kvh, uint64_t total, uint32_t 
 }
 
 // Splits for at most one workgroup a CU (tree_mfma, whose records grow with the
-// splits: 64 rows over 8192 positions 18.9 us, 23.1 with two a CU) or two
+// splits: 64 rows over 8192 positions 19.0 us, 23.1 with two a CU) or two
 // (tree_rows: 97 us against 109 with one at 1024 rows over 8256).  At most: one
 // workgroup too many is a second round for all (80 rows over 8192 positions
 // 21.7 us with 240 workgroups, 26.8 with 264).
@@ -1170,7 +1172,7 @@ static void launch_tree(const TreeArgs& a, hipStream_t st) {
     }
   } else {
     if constexpr (HD <= 128) {
-      if (p.tiles == 2) RF_KLAUNCH((tree_mfma<T, HD, 2>), grid, wg, 0, st, a);
+      if (p.tiles == 2) RF_KLAUNCH((tree_mfma<T, HD, 2>), grid, dim3(64 * tree_wide(T, HD, 2)), 0, st, a);
     }
     if (p.tiles == 1) RF_KLAUNCH((tree_mfma<T, HD, 1>), grid, wg, 0, st, a);
   }
