@@ -290,12 +290,12 @@ int32_t rf_attention_decode_noalloc(rf_ctx *ctx, const float *q, const float *k_
  *     -127..127 (-8..7).  Larger magnitudes than 65024 (65280) are cut there;
  *     a block of 32 that holds an infinity or NaN reads back as NaN.
  *     Not the GGUF block layout.
- * head_dim is at most 512; the buffers are 16-byte aligned.  `length`, if not
- * NULL, is a device word that every call adds to the positions it is given
- * (first, hist_len, src), read when the call runs: a captured graph then
- * follows a cache that grows.  The sum is checked on the device: rows past
- * the capacity are neither written, read nor seen (rf_kv_load leaves their
- * outputs as they are). */
+ * head_dim is at most 512, kv_heads at most 65535 and a position at most 2^20
+ * values; the buffers are 16-byte aligned.  `length`, if not NULL, is a device
+ * word that every call adds to the positions it is given (first, hist_len,
+ * src), read when the call runs: a captured graph then follows a cache that
+ * grows.  The sum is checked on the device: rows past the capacity are neither
+ * written, read nor seen (rf_kv_load leaves their outputs as they are). */
 typedef struct {
     uint32_t type; /* RF_TYPE_F32, RF_TYPE_F16, RF_TYPE_Q8_0 or RF_TYPE_Q4_0 */
     uint32_t kv_heads;
@@ -355,9 +355,9 @@ int32_t rf_tree_mask(rf_ctx *ctx, const int32_t *parents, uint64_t n, uint64_t b
  * hist_len .. hist_len + n - 1: each sees positions 0 .. hist_len - 1, and of
  * the n those whose bits its row of mask has (device memory, laid out as
  * above; NULL: a chain, tokens 0..i; n = 1 without a mask is rf_attention_decode
- * over such a cache).  q and out are [n][q_heads][head_dim]; scores are over
+ * over such a cache).  n times the query heads of a KV head is at most 65535 * 16.  q and out are [n][q_heads][head_dim]; scores are over
  * sqrt(head_dim), products and sums to f32 accuracy whatever the cache holds.
- * A token that sees nothing, or only scores of minus infinity, gets zeros.
+ * A token that sees nothing, or only scores below -2e38, gets zeros.
  * What positions hold that a token does not see cannot reach it, infinities
  * and NaN included; an infinity or NaN that it does see makes its output NaN
  * or infinite.  Uses the attention workspace: rf_attention_tree_workspace_bytes

@@ -505,14 +505,18 @@ class KvCache:
         return self.n_kv_heads * self.head_dim
 
     def free(self) -> None:
-        """Frees the buffers this object allocated."""
+        """Frees the buffers this object allocated; calls then refuse the cache."""
         for b in self.owned:
             b.free()
+            if b is self.k:
+                self.struct.k = None
+            if b is self.v:
+                self.struct.v = None
         self.owned = []
 
 
 class KvCacheList:
-    """The caches of a model's layers, for kv_move."""
+    """The caches of a model's layers, for kv_move; they must outlive it."""
 
     def __init__(self, caches: Sequence[KvCache]):
         self.caches = list(caches)

@@ -38,7 +38,7 @@ int32_t check_cache(const char* op, const rf_kv_cache* c, KvView* out) {
     return set_error(RF_ERR_UNSUPPORTED, "%s does not support a cache of tensor type %s (%u)", op, type_name(c->type), c->type);
   if (c->kv_heads == 0 || c->head_dim == 0 || c->capacity == 0)
     return set_error(RF_ERR_INVALID, "%s requires a cache of non-zero positions, KV heads and head dimension", op);
-  if (c->head_dim > KV_MAX_HEAD_DIM || c->kv_heads > 65535u)
+  if (c->head_dim > KV_MAX_HEAD_DIM || c->kv_heads > 65535u || (uint64_t)c->kv_heads * c->head_dim > KV_MAX_WIDTH)
     return set_error(RF_ERR_UNSUPPORTED, "%s does not cover %u KV heads of %u", op, c->kv_heads, c->head_dim);
   if (c->type >= RF_TYPE_Q4_0 && c->head_dim % 32)
     return set_error(RF_ERR_INVALID, "%s cache head_dim %u not divisible by 32", cache_type_name(c->type), c->head_dim);
@@ -85,7 +85,7 @@ extern "C" {
 uint64_t rf_kv_cache_bytes(uint32_t type, uint64_t capacity, uint32_t kv_heads, uint32_t head_dim) {
   uint64_t all = 0;
   if (!cache_type_name(type) || (type >= RF_TYPE_Q4_0 && head_dim % 32) || kv_heads > 65535u ||
-      head_dim > KV_MAX_HEAD_DIM || capacity > 0xFFFFFFFFull)
+      head_dim > KV_MAX_HEAD_DIM || (uint64_t)kv_heads * head_dim > KV_MAX_WIDTH || capacity > 0xFFFFFFFFull)
     return 0;
   return mul_ok(capacity, kv_row_bytes(type, (uint64_t)kv_heads * head_dim), &all) ? all : 0;
 }
@@ -218,7 +218,8 @@ int32_t rf_tree_mask(rf_ctx* ctx, const int32_t* parents, uint64_t n, uint64_t b
 uint64_t rf_attention_tree_workspace_bytes(uint64_t max_positions, uint64_t n, uint32_t type, uint32_t qh, uint32_t kvh,
                                            uint32_t hd) {
   if (max_positions == 0 || n == 0 || qh == 0 || kvh == 0 || hd == 0 || n > TREE_MAX_NODES || qh % kvh ||
-      !cache_type_name(type) || max_positions > 0xFFFFFFFFull || qh > 65535u || hd > KV_MAX_HEAD_DIM)
+      !cache_type_name(type) || max_positions > 0xFFFFFFFFull || qh > 65535u || hd > KV_MAX_HEAD_DIM ||
+      n * (qh / kvh) > TREE_MAX_ROWS)
     return 0;
   return tree_ws_floats_upto(max_positions, (uint32_t)n, qh, kvh, hd, type) * 4;
 }
@@ -235,6 +236,9 @@ int32_t rf_attention_tree(rf_ctx* ctx, const float* q, uint64_t q_stride, const 
   if (n > TREE_MAX_NODES || q_heads > 65535u)
     return set_error(RF_ERR_UNSUPPORTED, "tree attention does not cover %llu tokens of %u query heads (at most %u)",
                      (ull)n, q_heads, TREE_MAX_NODES);
+  if (n * (q_heads / a.cache.kvh) > TREE_MAX_ROWS)
+    return set_error(RF_ERR_UNSUPPORTED, "tree attention does not cover %llu tokens of %u query heads a KV head",
+                     (ull)n, q_heads / a.cache.kvh);
   RF_TRY(check_rows("tree attention", a.cache, hist_len, n));
   const uint64_t width = (uint64_t)q_heads * a.cache.hd;
   RF_TRY(check_stride("tree attention", "q", &q_stride, width, n));

@@ -11,7 +11,7 @@ namespace rf {
 // one f16 scale per 32 values [cap][kvh * hd / 32]:
 //   Q8_0: a byte per value, code + 128, code in -127..127.  The scale is the
 //         least f16 of at most 3 significant bits with 127 d >= max |x|: a
-//         code has at most 7 bits and a sign, so code * d has at most 11 - 1
+//         code has at most 7 bits and a sign, so code * d has at most 10
 //         significant bits and is an f16 exactly.  The matrix cores then take
 //         the cached values themselves, and no scale is left for the scores.
 //         (Rounding the scale up costs 11% of a step on average, 25% at most;
@@ -34,6 +34,9 @@ constexpr uint32_t KV_MOVE_MAX = 1024;   // rows of one move
 constexpr uint32_t KV_MOVE_CACHES = 64;  // caches of one launch (pointers are kernel arguments)
 constexpr uint32_t TREE_MAX_NODES = 1024;
 constexpr uint32_t KV_MAX_HEAD_DIM = 512;
+// Values of a position, and rows (tokens times query heads) of a KV head: grids
+// and byte offsets within a tile stay inside 32 bits, grid y inside 16.
+constexpr uint32_t KV_MAX_WIDTH = 1u << 20, TREE_MAX_ROWS = 65535u * 16u;
 
 inline uint64_t kv_code_bytes(uint32_t type, uint64_t values) {
   return type == 0u ? values * 4 : type == 1u ? values * 2 : type == 8u ? values : values / 2;

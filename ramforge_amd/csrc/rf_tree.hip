@@ -97,7 +97,8 @@ __global__ __launch_bounds__(256) void tree_plain(TreeArgs a) {
   uint64_t hist, total;
   tree_range(a, hist, total);
   for (uint32_t d = tid; d < hd; d += 256u) qs[d] = a.q[(uint64_t)i * a.q_stride + (uint64_t)h * hd + d];
-  float o[2] = {0.f, 0.f}, m = -INFINITY, l = 0.f;
+  double o[2] = {0., 0.}, l = 0.;
+  float m = -INFINITY;
   const float denom = sqrtf((float)hd);
   for (uint64_t p0 = 0; p0 < total; p0 += 256u) {
     const uint64_t pos = p0 + tid;
@@ -122,17 +123,17 @@ __global__ __launch_bounds__(256) void tree_plain(TreeArgs a) {
     __syncthreads();
     if ((tid & 63u) == 0u) red[tid >> 6] = ws;
     __syncthreads();
-    l = l * al + ((red[0] + red[1]) + (red[2] + red[3]));
+    l = l * al + (double)((red[0] + red[1]) + (red[2] + red[3]));
     const uint32_t np = (uint32_t)min((uint64_t)256u, total - p0);
     for (uint32_t r = 0, d = tid; d < hd; d += 256u, ++r) {
-      float acc = o[r] * al;
+      float acc = 0.f;
       for (uint32_t j = 0; j < np; ++j)
         if (seen[j]) acc = fmaf(p[j], kv_value(a.cache.v, a.cache, p0 + j, g * hd + d), acc);
-      o[r] = acc;
+      o[r] = o[r] * al + acc;
     }
   }
   for (uint32_t r = 0, d = tid; d < hd; d += 256u, ++r)
-    a.out[(uint64_t)i * a.out_stride + (uint64_t)h * hd + d] = l == 0.f ? 0.f : o[r] / l;
+    a.out[(uint64_t)i * a.out_stride + (uint64_t)h * hd + d] = l == 0. ? 0.f : (float)(o[r] / l);
 }
 
 // ---------------------------------------------------------- matrix cores

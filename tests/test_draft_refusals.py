@@ -26,6 +26,8 @@ BAD_CACHES = [
     (dict(head_dim=0), INVALID, "non-zero"),
     (dict(capacity=0), INVALID, "non-zero"),
     (dict(head_dim=544), UNSUPPORTED, "does not cover"),
+    (dict(kv_heads=65536), UNSUPPORTED, "does not cover"),
+    (dict(kv_heads=8193, head_dim=128), UNSUPPORTED, "does not cover"),
     (dict(head_dim=80), INVALID, "not divisible by 32"),
     (dict(type=2, head_dim=16), INVALID, "Q4_0 cache head_dim 16 not divisible by 32"),
     (dict(capacity=1 << 32), UNSUPPORTED, "2^32 - 1"),
@@ -185,3 +187,33 @@ def test_tree_workspace_bytes():
             now = lib.rf_attention_tree_workspace_bytes(9000, n, t, 32, 8, 128)
             assert now >= last
             last = now
+
+
+def test_widest_positions():
+    lib = _lib.load()
+    assert lib.rf_kv_cache_bytes(1, 10, 8192, 128) == 10 * 2 ** 20 * 2
+    assert lib.rf_kv_cache_bytes(1, 10, 8193, 128) == 0
+    one = cache(type=1, kv_heads=1, head_dim=64, capacity=5000)
+    refused(lib.rf_attention_tree(CTX, P, 0, one, 0, None, 1024, 1024, P, 0, None), UNSUPPORTED,
+            "does not cover 1024 tokens of 1024 query heads a KV head")
+    assert lib.rf_attention_tree_workspace_bytes(5000, 1024, 1, 1024, 1, 64) == 0
+
+
+def test_a_freed_cache_is_refused():
+    import ramforge_amd as rf
+
+    class Ctx:
+        handle, lib = CTX, _lib.load()
+
+    class Buffer(rf.DeviceArray):
+        def free(self):
+            self.ptr = 0
+
+    k, v = (Buffer(Ctx, P, 1 << 20, (1 << 20,), "uint8", "") for _ in range(2))
+    c = rf.KvCache(Ctx, 8, 100, 2, 64, k, v)
+    c.owned = [k, v]
+    c.free()
+    with pytest.raises(rf.RamforgeError, match="null buffer"):
+        rf.kv_store(Ctx, c, P, P, 0, 1)
+    with pytest.raises(rf.RamforgeError, match="null buffer"):
+        rf.kv_move(Ctx, [c], P, 0, 1)
