@@ -209,17 +209,29 @@ __device__ __forceinline__ void tree_bytes(uint32_t* w, TreeRsrc r, uint32_t off
 __device__ __forceinline__ uint32_t pk_mul(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, a) * __builtin_bit_cast(half2_t, b));
 }
-// (x | magic) is an f16 pair of `one` + codes with their offset; minus that it is the codes.
-__device__ __forceinline__ uint32_t pk_code(uint32_t x, uint32_t mask, uint32_t magic, float off) {
+// What decoding takes: (x & mask) | magic is an f16 pair of `one` + codes with
+// their offset, and minus that it is the codes.  The masks are scalars and the
+// magics vector registers that the compiler does not know to be constants: as
+// literals the two operations would not be one instruction (64 of the 408 of a
+// tile of Q4_0 with two row tiles).
+struct TreeMagic {
+  uint32_t low = 0x000F000Fu, high = 0x00F000F0u, m64 = 0x64006400u, m54 = 0x54005400u;
+  __device__ __forceinline__ TreeMagic() {
+    asm("" : "+s"(low));
+    asm("" : "+s"(high));
+    asm("" : "+v"(m64));
+    asm("" : "+v"(m54));
+  }
+};
+__device__ __forceinline__ uint32_t pk_minus(uint32_t x, float off) {
   const half2_t o = {(_Float16)off, (_Float16)off};
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, (x & mask) | magic) - o);
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, x) - o);
 }
-__device__ __forceinline__ uint32_t pk_q8(uint32_t x) { return pk_code(x, 0x00FF00FFu, 0x64006400u, 1152.f); }
 // Nibble k (0..3) of both halves of x.
 template <int K>
-__device__ __forceinline__ uint32_t pk_q4(uint32_t x) {
+__device__ __forceinline__ uint32_t pk_q4(uint32_t x, const TreeMagic& mg) {
   if constexpr (K >= 2) x >>= 8;
-  return K % 2 ? pk_code(x, 0x00F000F0u, 0x54005400u, 72.f) : pk_code(x, 0x000F000Fu, 0x64006400u, 1032.f);
+  return K % 2 ? pk_minus((x & mg.high) | mg.m54, 72.f) : pk_minus((x & mg.low) | mg.m64, 1032.f);
 }
 
 // One tile of 32 positions as a lane holds it, and its decoding.
@@ -271,34 +283,35 @@ template <uint32_t T, int HD> struct TreeTile {
   static __device__ __forceinline__ constexpr int order(int i) { return T == T_Q4_0 ? (i / 2) + 4 * (i % 2) : i; }
 
   // The eight halves of a step's K words.
-  static __device__ __forceinline__ void decode_k(const uint32_t* k, uint32_t scale, u32x4& w) {
+  static __device__ __forceinline__ void decode_k(const uint32_t* k, uint32_t scale, const TreeMagic& mg, u32x4& w) {
     const uint32_t s2 = scale | scale << 16;
     if constexpr (T == T_Q8_0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        w[2 * i] = pk_mul(pk_q8(__builtin_amdgcn_perm(0u, k[i], 0x0C010C00u)), s2);
-        w[2 * i + 1] = pk_mul(pk_q8(__builtin_amdgcn_perm(0u, k[i], 0x0C030C02u)), s2);
+        w[2 * i] = pk_mul(pk_minus(__builtin_amdgcn_perm(mg.m64, k[i], 0x05010500u), 1152.f), s2);
+        w[2 * i + 1] = pk_mul(pk_minus(__builtin_amdgcn_perm(mg.m64, k[i], 0x05030502u), 1152.f), s2);
       }
     } else {
-      w[0] = pk_mul(pk_q4<0>(k[0]), s2);
-      w[1] = pk_mul(pk_q4<1>(k[0]), s2);
-      w[2] = pk_mul(pk_q4<2>(k[0]), s2);
-      w[3] = pk_mul(pk_q4<3>(k[0]), s2);
+      w[0] = pk_mul(pk_q4<0>(k[0], mg), s2);
+      w[1] = pk_mul(pk_q4<1>(k[0], mg), s2);
+      w[2] = pk_mul(pk_q4<2>(k[0], mg), s2);
+      w[3] = pk_mul(pk_q4<3>(k[0], mg), s2);
     }
   }
-  __device__ __forceinline__ half8_t kfrag(int t, int s) const {
+  __device__ __forceinline__ half8_t kfrag(int t, int s, const TreeMagic& mg) const {
     u32x4 w;
     if constexpr (T == T_F16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = k[t][4 * s + i];
     } else {
-      decode_k(k[t] + s * (BITS / 4), ks[t][HD == 96 ? s : s / 4], w);
+      decode_k(k[t] + s * (BITS / 4), ks[t][HD == 96 ? s : s / 4], mg, w);
     }
     return __builtin_bit_cast(half8_t, w);
   }
   // The halves of two positions a, b at dim TILE of the lane's
   template <int TILE>
-  static __device__ __forceinline__ uint32_t pair(const uint32_t* va, const uint32_t* vb, const uint32_t* sa, const uint32_t* sb) {
+  static __device__ __forceinline__ uint32_t pair(const uint32_t* va, const uint32_t* vb, const uint32_t* sa,
+                                                  const uint32_t* sb, const TreeMagic& mg) {
     constexpr int seg = TILE < D::W0 ? 0 : 1, e = seg ? TILE - D::W0 : TILE, per = 32 / BITS;  // element e of the lane's dims
     constexpr int word = (seg ? VW0 : 0) + e / per, in = e % per;
     const uint32_t a = va[word], b = vb[word];
@@ -307,28 +320,28 @@ template <uint32_t T, int HD> struct TreeTile {
     } else {
       const uint32_t s2 = sa[seg] | sb[seg] << 16;
       if constexpr (T == T_Q8_0) {
-        return pk_mul(pk_q8(__builtin_amdgcn_perm(b, a, 0x0C040C00u + 0x00010001u * in)), s2);
+        return pk_mul(pk_minus(__builtin_amdgcn_perm(b, a, 0x0C040C00u + 0x00010001u * in) | mg.m64, 1152.f), s2);
       } else {
         const uint32_t x = __builtin_amdgcn_perm(b, a, in < 4 ? 0x05040100u : 0x07060302u);
-        return pk_mul(pk_q4<in % 4>(x), s2);
+        return pk_mul(pk_q4<in % 4>(x, mg), s2);
       }
     }
   }
   // V^T's tile of 16 dims
   template <int TILE>
-  __device__ __forceinline__ half8_t vfrag() const {
+  __device__ __forceinline__ half8_t vfrag(const TreeMagic& mg) const {
     u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pair<TILE>(v[2 * i], v[2 * i + 1], vs[2 * i], vs[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) w[i] = pair<TILE>(v[2 * i], v[2 * i + 1], vs[2 * i], vs[2 * i + 1], mg);
     return __builtin_bit_cast(half8_t, w);
   }
   // One word of all tiles' operands, from two positions
   template <int TILE = 0>
   static __device__ __forceinline__ void decode_v(const uint32_t* va, const uint32_t* vb, const uint32_t* sa,
-                                                  const uint32_t* sb, uint32_t (&w)[D::TILES]) {
+                                                  const uint32_t* sb, const TreeMagic& mg, uint32_t (&w)[D::TILES]) {
     if constexpr (TILE < D::TILES) {
-      w[TILE] = pair<TILE>(va, vb, sa, sb);
-      decode_v<TILE + 1>(va, vb, sa, sb, w);
+      w[TILE] = pair<TILE>(va, vb, sa, sb, mg);
+      decode_v<TILE + 1>(va, vb, sa, sb, mg, w);
     }
   }
 };
@@ -588,7 +601,7 @@ __device__ __forceinline__ half8_t tree_finite(half8_t v, bool& odd) {
 // sum before it.  DRAFTS: non-finite values are taken out (see above).
 template <uint32_t T, int HD, int M, bool DRAFTS, int TILE>
 __device__ __forceinline__ void tree_tiles(const TreeTile<T, HD>& x, const u32x4 (&ph)[M], const u32x4 (&pl)[M],
-                                           bool& odd, f32x4 (&o)[M][TreeDims<HD>::TILES]) {
+                                           const TreeMagic& mg, bool& odd, f32x4 (&o)[M][TreeDims<HD>::TILES]) {
   constexpr int N = M == 1 ? 4 : 2;
   static_assert(TreeDims<HD>::TILES % 2 == 0, "whole groups");
   if constexpr (TILE < TreeDims<HD>::TILES) {
@@ -596,7 +609,7 @@ __device__ __forceinline__ void tree_tiles(const TreeTile<T, HD>& x, const u32x4
     auto decode = [&](auto i) {
       constexpr int I = decltype(i)::value;
       if constexpr (I < N && TILE + I < TreeDims<HD>::TILES) {
-        vf[I] = x.template vfrag<TILE + I>();
+        vf[I] = x.template vfrag<TILE + I>(mg);
         if constexpr (DRAFTS) vf[I] = tree_finite(vf[I], odd);
       }
     };
@@ -614,7 +627,7 @@ __device__ __forceinline__ void tree_tiles(const TreeTile<T, HD>& x, const u32x4
             o[m][TILE + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                 vf[i], __builtin_bit_cast(half8_t, piece ? ph[m] : pl[m]), o[m][TILE + i], 0, 0, 0);
         }
-    tree_tiles<T, HD, M, DRAFTS, TILE + N>(x, ph, pl, odd, o);
+    tree_tiles<T, HD, M, DRAFTS, TILE + N>(x, ph, pl, mg, odd, o);
   }
 }
 
@@ -687,6 +700,7 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
   float scale[M], ref[M], l[M];
   f32x4 o[M][D::TILES];
   const float minus = tree_minus();
+  const TreeMagic mg;
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     tok[m] = min(row0 + 16u * m + c, rows - 1u) / G;
@@ -699,6 +713,7 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
 
   auto step = [&](auto drafts) {
     constexpr bool DRAFTS = decltype(drafts)::value;  // the tile has positions that some rows may not see
+    __builtin_amdgcn_s_setprio(0);
     const uint64_t p0 = (uint64_t)tile * TREE_KEYS;
     // scores of row c at positions p0 + 16 t + 4 g + v
     f32x4 s[M][2];
@@ -720,7 +735,7 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
     } else {
 #pragma unroll
       for (int i = 0; i < D::STEPS; ++i) {
-        const half8_t k0 = cur.kfrag(0, i), k1 = cur.kfrag(1, i);
+        const half8_t k0 = cur.kfrag(0, i, mg), k1 = cur.kfrag(1, i, mg);
 #pragma unroll
         for (int piece = 0; piece < 2; ++piece)
 #pragma unroll
@@ -733,6 +748,9 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
     }
     __builtin_amdgcn_sched_barrier(0);
     fetch_k(tile + W);  // the old words are spent
+    // ahead of a wavefront that is at its scores: the two of a SIMD stay apart,
+    // one at vector instructions while the other feeds the matrix cores (1 to 2%)
+    __builtin_amdgcn_s_setprio(1);
     float p[M][8];
     uint32_t see[M];
 #pragma unroll
@@ -765,7 +783,7 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
           ph[m][j] = h;
           pl[m][j] = r;
         }
-      tree_tiles<T, HD, M, DRAFTS, 0>(cur, ph, pl, odd, o);
+      tree_tiles<T, HD, M, DRAFTS, 0>(cur, ph, pl, mg, odd, o);
     }
     __builtin_amdgcn_sched_barrier(0);
     fetch_v(tile + W);
@@ -775,6 +793,7 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
   for (; tile < t1 && (uint64_t)tile * TREE_KEYS + TREE_KEYS <= hist; tile += W) step(std::false_type());
   for (; tile < t1; tile += W) step(std::true_type());
 
+  __builtin_amdgcn_s_setprio(0);
   // Join the wavefronts: all their sums in LDS (in Q's place, so once all are
   // done with it), and what a sum weighs is worked out where it is added.
   __syncthreads();
@@ -862,13 +881,13 @@ template <uint32_t T, int HD> struct TreePart {
       }
     }
   }
-  __device__ __forceinline__ half8_t kfrag(int s) const {
+  __device__ __forceinline__ half8_t kfrag(int s, const TreeMagic& mg) const {
     u32x4 w;
     if constexpr (T == T_F16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = k[4 * s + i];
     } else {
-      Tile::decode_k(k + s * SW, ks[HD == 96 ? s : 0], w);
+      Tile::decode_k(k + s * SW, ks[HD == 96 ? s : 0], mg, w);
     }
     return __builtin_bit_cast(half8_t, w);
   }
@@ -910,13 +929,14 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a) {
                 head, c, g, wave);
     __builtin_amdgcn_sched_barrier(0);
   };
+  const TreeMagic mg;
   auto put = [&](uint32_t buf) {
     const uint32_t t = wave & 1u, s0 = (wave >> 1) * Part::KSTEPS;
 #pragma unroll
     for (int i = 0; i < Part::KSTEPS; ++i)
-      if (D::STEPS % 2 == 0 || s0 + i < (uint32_t)D::STEPS) sh.k[buf][t][s0 + i][lane] = __builtin_bit_cast(u32x4, part.kfrag(i));
+      if (D::STEPS % 2 == 0 || s0 + i < (uint32_t)D::STEPS) sh.k[buf][t][s0 + i][lane] = __builtin_bit_cast(u32x4, part.kfrag(i, mg));
     uint32_t w[D::TILES];
-    Tile::decode_v(part.v[0], part.v[1], part.vs[0], part.vs[1], w);
+    Tile::decode_v(part.v[0], part.v[1], part.vs[0], part.vs[1], mg, w);
 #pragma unroll
     for (int d = 0; d < D::TILES; ++d) reinterpret_cast<uint32_t*>(&sh.v[buf][d][lane])[wave] = w[d];
   };
