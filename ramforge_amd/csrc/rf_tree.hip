@@ -401,8 +401,8 @@ __device__ __forceinline__ void tree_pieces(float x, float y, float minus, uint3
 constexpr uint32_t TREE_ODD = 36;
 // Wavefronts of a workgroup of tree_mfma: eight (two a SIMD, one decoding under
 // the other's matrix instructions) where two row tiles keep a CU to itself, four
-// where workgroups are many and small (128 rows over 8192 positions 25.4 us with
-// four, 22.7 with eight; one token over 2048 9.8 and 10.2).
+// where workgroups are many and small (1024 rows over 8256 positions 93 us with
+// four, 83 with eight; one token over 2048 9.8 and 10.2).
 constexpr int tree_wide(uint32_t type, int hd, int m) { return m == 2 && !(type == T_F32 && hd == 128) ? 8 : 4; }
 template <uint32_t T, int HD, int M> struct TreeShared {
   static constexpr int W = tree_wide(T, HD, M);
@@ -972,6 +972,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a) {
 
   auto step = [&](auto drafts, uint32_t tile, uint32_t buf) {
     constexpr bool DRAFTS = decltype(drafts)::value;
+    __builtin_amdgcn_s_setprio(0);
     const uint64_t p0 = (uint64_t)tile * TREE_KEYS;
     f32x4 s[M][2];
 #pragma unroll
@@ -987,6 +988,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a) {
           s[m][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, piece ? qh[m][i] : ql[m][i], s[m][1], 0, 0, 0);
         }
     }
+    __builtin_amdgcn_s_setprio(1);  // as in tree_mfma
     float p[M][8];
     uint32_t see[M];
     u32x4 ph[M], pl[M];
@@ -1118,14 +1120,15 @@ static bool tree_on_matrix_cores(uint32_t hd) { return hd == 64 || hd == 96 || h
 // few records to join; tree_rows, whose wavefronts split the rows, decodes less
 // and reads the cache fewer times.  The first is ahead until every CU has 5 hd
 // pairs of a row tile and a tile of positions (us in the first and the second,
-// 8 KV heads of 128: 64 rows over 8192 Q8_0 positions 18.7 and 27.8, 256 over
-// 8192 31.5 and 49.4, 1024 over 8256 86 and 94, 64 over 131072 Q4_0 positions
-// 92 and 96, 512 over 32128 163 and 143; 2 of 64, 1400 rows over 16200 F16
-// positions 52 and 45).  An f32 cache has nothing to decode and stays with it.
+// 8 KV heads of 128: 64 rows over 8192 Q8_0 positions 18.3 and 27.2, 256 over
+// 8192 31.0 and 47.8, 1024 over 8256 84 and 95, 512 over 16128 85.9 and 87.8,
+// 64 over 131072 Q4_0 positions 89.7 and 96.1, 256 over 65600 155 and 144, 512
+// over 32128 Q8_0 positions 160 and 141; 2 of 64, 1400 rows over 8200 F16
+// positions 30.8 and 33.4, over 16200 51.4 and 45.6).  An f32 cache has nothing to decode and stays with it.
 //
 // Row tiles of a wavefront in the first: two where that leaves a workgroup for
-// every CU, one otherwise (37 tokens over 637 f32 positions: 13.2 us with one,
-// 17.8 with two).
+// every CU, one otherwise (37 tokens over 637 f32 positions: 12.3 us with one,
+// 16.7 with two; 1024 rows over 8256 Q8_0 positions 133 and 83).
 struct TreePlan {
   bool rows_apart;
   uint32_t tiles, block_rows;  // row tiles of a wavefront, rows of a workgroup
@@ -1146,10 +1149,10 @@ static TreePlan tree_plan(uint64_t rows, uint32_t kvh, uint64_t total, uint32_t 
 }
 
 // Splits for at most one workgroup a CU (tree_mfma, whose records grow with the
-// splits: 64 rows over 8192 positions 19.0 us, 23.1 with two a CU) or two
-// (tree_rows: 97 us against 109 with one at 1024 rows over 8256).  At most: one
+// splits: 64 rows over 8192 positions 18.0 us, 26.3 with two a CU) or two
+// (tree_rows: 141 us against 160 with one at 512 rows over 32128).  At most: one
 // workgroup too many is a second round for all (80 rows over 8192 positions
-// 21.7 us with 240 workgroups, 26.8 with 264).
+// 20.4 us with 240 workgroups, 28.2 with 264).
 uint32_t tree_splits(uint64_t total, uint32_t n, uint32_t qh, uint32_t kvh, uint32_t hd, uint32_t type) {
   if (!tree_on_matrix_cores(hd)) return 1;
   const uint64_t rows = (uint64_t)n * (qh / kvh);
