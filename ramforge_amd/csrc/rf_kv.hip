@@ -181,7 +181,8 @@ __device__ __forceinline__ RowMap row_map(const KvView& c) {
 // flight: a thread asks for U rows before it uses the first, with addresses
 // clamped instead of branches (a load in a branch is waited for there).  8191
 // rows of 1024 values into Q4_0, 76 MB: 25.8 us with the exact rounding for
-// every value, 21.4 us without it and one row a thread.
+// every value, 21.4 us without it and one row a thread, 19.2 us as it is (4.0
+// TB/s); back to floats 13.2 us.
 template <bool LOAD, uint32_t T, int U>
 __global__ __launch_bounds__(256) void kv_rows(KvView c, float* k, uint64_t k_stride, float* v, uint64_t v_stride,
                                                uint64_t first, uint64_t n) {
@@ -307,7 +308,8 @@ struct MoveArgs {
 
 // A workgroup takes `slice` units of every row of one buffer: all its reads
 // are in LDS before its first write, so a row may be source and target, in
-// any order.
+// any order.  Bound by its launch and one round trip to HBM: 32 layers of 5 F16
+// rows 4.0 us, 28 layers of 100 F32 rows (11.5 MB) 6.4 us.
 template <typename U>
 __global__ __launch_bounds__(256) void kv_move(MoveArgs a) {
   __shared__ U held[KV_MOVE_MAX];

@@ -164,6 +164,13 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // row to 2^10 .. 2^11) and P (up to 2^15) are taken as two f16 pieces, 22 bits
 // together, products and sums in f32.  An f32 cache takes f32 matrix
 // instructions, 1/16 of the f16 rate (1/8 for the two pieces).
+//
+// Bound by vector issue where positions are many (a matrix instruction keeps a
+// SIMD's vector issue for about half its 16 cycles, and a tile of Q4_0 with two
+// row tiles takes 344 vector instructions beside 64 of them): 1024 rows over
+// 8256 Q8_0 positions 82 us, 0.84 PFLOP/s of matrix work; 64 over 131072 Q4_0
+// 88 us.  By the start, the first tile's loads and the join where they are few:
+// 64 rows over 8192 Q8_0 positions 17.3 us with tree_join's 4.0.
 template <int HD> struct TreeDims {
   static constexpr int STEPS = HD / 32;   // matrix instructions of a half tile's scores
   static constexpr int TILES = HD / 16;   // 16-dim tiles of the output
@@ -848,6 +855,8 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
 // same positions, each decodes a quarter of a tile into LDS as the matrix
 // instructions take it, and all read it from there.  Tiles are double-buffered:
 // one barrier each; the words of the next but one are in flight.
+// 512 rows over 32128 Q8_0 positions 141 us, 0.96 PFLOP/s; bound by the chain of
+// a tile (LDS reads, scores, softmax, sums) with two wavefronts a SIMD.
 //   Wavefront w decodes, of K, half tile w % 2 and steps from w / 2 (STEPS / 2
 //   rounded up), and of V its positions 4 t + v = 2 w, 2 w + 1 for all dims:
 //   word w of every tile's operand.
@@ -1070,7 +1079,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a) {
 }
 
 // Joins a row's records: HD / 4 lanes of 4 dims take every JOIN-th split, and
-// their sums meet in LDS, so that a row of many splits is a few loads deep.
+// their sums meet in LDS, so that a row of many splits is a few loads deep.  3.0
+// us for 32 rows, 4.0 for 512 of 16 splits; a launch alone is 2.6.
 template <int HD>
 __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
   constexpr uint32_t LANES = HD / 4, JOIN = 256u / LANES;
@@ -1124,7 +1134,8 @@ static bool tree_on_matrix_cores(uint32_t hd) { return hd == 64 || hd == 96 || h
 // 8192 31.0 and 47.8, 1024 over 8256 84 and 95, 512 over 16128 85.9 and 87.8,
 // 64 over 131072 Q4_0 positions 89.7 and 96.1, 256 over 65600 155 and 144, 512
 // over 32128 Q8_0 positions 160 and 141; 2 of 64, 1400 rows over 8200 F16
-// positions 30.8 and 33.4, over 16200 51.4 and 45.6).  An f32 cache has nothing to decode and stays with it.
+// positions 30.8 and 33.4, over 16200 51.4 and 45.6).  An f32 cache has nothing
+// to decode and stays with it.
 //
 // Row tiles of a wavefront in the first: two where that leaves a workgroup for
 // every CU, one otherwise (37 tokens over 637 f32 positions: 12.3 us with one,
