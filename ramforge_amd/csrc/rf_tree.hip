@@ -170,7 +170,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // row tiles takes 344 vector instructions beside 64 of them): 1024 rows over
 // 8256 Q8_0 positions 82 us, 0.84 PFLOP/s of matrix work; 64 over 131072 Q4_0
 // 88 us.  By the start, the first tile's loads and the join where they are few:
-// 64 rows over 8192 Q8_0 positions 17.3 us with tree_join's 4.0.
+// 64 rows over 8192 Q8_0 positions 17.1 us with tree_join.
 template <int HD> struct TreeDims {
   static constexpr int STEPS = HD / 32;   // matrix instructions of a half tile's scores
   static constexpr int TILES = HD / 16;   // 16-dim tiles of the output
@@ -260,10 +260,12 @@ template <uint32_t T, int HD> struct TreeTile {
                                          uint32_t c, uint32_t g) {
     const uint32_t hb = head * (HD * BITS / 8), hs = head * (HD / 16);
 #pragma unroll
-    for (uint32_t t = 0; t < 2; ++t) {
-      const uint32_t p = 16u * t + c;
-      tree_words<KW>(k[t], kr, p * row + hb + g * (KW * 4u));
-      if constexpr (QUANT) {
+    for (uint32_t t = 0; t < 2; ++t) tree_words<KW>(k[t], kr, (16u * t + c) * row + hb + g * (KW * 4u));
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (QUANT) {
+#pragma unroll
+      for (uint32_t t = 0; t < 2; ++t) {
+        const uint32_t p = 16u * t + c;
 #pragma unroll
         for (uint32_t i = 0; i < (uint32_t)KS; ++i) {
           const uint32_t b = HD == 96 ? (g * 24u + 8u * i) / 32u : HD == 64 ? g / 2u : g * (HD / 128) + i;
@@ -644,7 +646,9 @@ constexpr int tree_waves_per_simd(uint32_t type, int hd, int m) {
   return (type == T_F32 && hd * m >= 256) || (hd == 256 && (type == T_F16 || type == T_Q8_0)) || hd * m > 256 ? 1 : 2;
 }
 template <uint32_t T, int HD, int M>
-__global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 ? 1 : tree_waves_per_simd(T, HD, M)) void tree_mfma(TreeArgs a) {
+__global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 ? 1 : tree_waves_per_simd(T, HD, M)) void tree_mfma(
+    const float* q, uint64_t q_stride, const uint8_t* k_codes, const uint32_t* length, uint32_t rows, uint32_t G,
+    uint32_t row, uint32_t all_tiles, uint32_t all_per, uint32_t all_total, TreeArgs a) {
   using D = TreeDims<HD>;
   using Tile = TreeTile<T, HD>;
   using S = TreeShared<T, HD, M>;
@@ -654,28 +658,28 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
   const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: the tiles' descriptors are scalars
   const uint32_t split = blockIdx.x, head = blockIdx.z, row0 = blockIdx.y * (M * 16u);
-  const uint32_t G = a.group, rows = a.rows, words = a.words;
+  const uint32_t words = a.words;
 
   // this lane's Q: wavefront w has row tiles w, w + 4, ..; requested before the cache's rows
   float x[HD / 4];
   auto ask_q = [&](int m) {
     const uint32_t r = min(row0 + 16u * m + c, rows - 1u), i = r / G;
-    const float* const qp = a.q + (uint64_t)i * a.q_stride + ((uint64_t)head * G + (r - i * G)) * HD + g * (HD / 4);
+    const float* const qp = q + (uint64_t)i * q_stride + ((uint64_t)head * G + (r - i * G)) * HD + g * (HD / 4);
     tree_get_q<HD>(x, qp, a.q_vec);
   };
   static_assert(M <= (int)W, "a row tile per wavefront");
   if (wave < (uint32_t)M) ask_q((int)wave);
   __builtin_amdgcn_sched_barrier(0);
 
-  uint64_t hist = a.hist, total = a.total;
-  uint32_t tiles = a.tiles, per = a.per;
-  if (a.cache.length) {
+  uint64_t hist = a.hist, total = all_total;
+  uint32_t tiles = all_tiles, per = all_per;
+  if (length) {
     tree_range(a, hist, total);
     tiles = (uint32_t)((total + TREE_KEYS - 1u) / TREE_KEYS);
     per = (tiles + a.nsplit - 1u) / a.nsplit;
   }
   const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
-  const uint32_t row = a.code_row, srow = a.scale_row;
+  const uint32_t srow = a.scale_row;
   const uint64_t sbase = a.scale_base;
   Tile cur;
   // Bounded descriptors: rows behind the last read as zeros, and nothing is
@@ -686,7 +690,7 @@ __global__ __launch_bounds__(64 * tree_wide(T, HD, M), tree_wide(T, HD, M) == 8 
   auto fetch_k = [&](uint32_t tile) {
     const uint64_t p = (uint64_t)tile * TREE_KEYS;
     const uint32_t np = rows_of(tile);
-    cur.load_k(tree_rsrc(a.cache.k + p * row, np * row), tree_rsrc(a.cache.k + sbase + p * srow, np * srow), row, srow,
+    cur.load_k(tree_rsrc(k_codes + p * row, np * row), tree_rsrc(a.cache.k + sbase + p * srow, np * srow), row, srow,
                head, c, g);
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -1079,20 +1083,21 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void tree_rows(TreeArgs a) {
 }
 
 // Joins a row's records: HD / 4 lanes of 4 dims take every JOIN-th split, and
-// their sums meet in LDS, so that a row of many splits is a few loads deep.  3.0
-// us for 32 rows, 4.0 for 512 of 16 splits; a launch alone is 2.6.
+// their sums meet in LDS, so that a row of many splits is a few loads deep.  2.4
+// us for 32 rows, 4.8 for 512 of 16 splits.
 template <int HD>
-__global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
+__global__ __launch_bounds__(256) void tree_join(const float* ws, float* to, uint64_t out_stride,
+                                                 uint32_t n_rows, uint32_t qh, uint32_t nsplit) {
   constexpr uint32_t LANES = HD / 4, JOIN = 256u / LANES;
   __shared__ __align__(16) float y[JOIN][HD + 4];
-  const uint64_t rows = (uint64_t)a.n * a.qh, r = blockIdx.x;
+  const uint64_t rows = n_rows, r = blockIdx.x;
   const uint32_t part = threadIdx.x / LANES, d = threadIdx.x % LANES * 4u;
-  const float* const rec = a.ws + r * (HD + 4);
+  const float* const rec = ws + r * (HD + 4);
   const uint64_t step = rows * (HD + 4);
   if (part < JOIN) {
     float top = TREE_FLOOR, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (uint32_t s = part; s < a.nsplit; s += JOIN) {
+    for (uint32_t s = part; s < nsplit; s += JOIN) {
       const float* const at = rec + s * step;
       const float4 z = *reinterpret_cast<const float4*>(at + d);
       const float m = at[HD], now = fmaxf(top, m), al = __builtin_amdgcn_exp2f(top - now), w = __builtin_amdgcn_exp2f(m - now);
@@ -1117,7 +1122,7 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
     o[0] = fmaf(z.x, w, o[0]); o[1] = fmaf(z.y, w, o[1]); o[2] = fmaf(z.z, w, o[2]); o[3] = fmaf(z.w, w, o[3]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  float* const out = a.out + r / a.qh * a.out_stride + r % a.qh * HD + d;
+  float* const out = to + r / qh * out_stride + r % qh * HD + d;
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = o[e] * inv;
 }
@@ -1194,6 +1199,12 @@ uint64_t tree_ws_floats_upto(uint64_t total, uint32_t n, uint32_t qh, uint32_t k
   return most;
 }
 
+// What a workgroup needs before its first load goes in front of the rest, as
+// scalars: the kernels of this file are built with their first 14 words of
+// arguments preloaded into registers, and do not wait for them (64 rows over
+// 8192 positions: tree_mfma 15.9 -> 14.9 us; the join of 32 rows 3.0 -> 2.4).
+#define TREE_FIRST \
+  a.q, a.q_stride, a.cache.k, a.cache.length, a.rows, a.group, a.code_row, a.tiles, a.per, (uint32_t)a.total
 template <uint32_t T, int HD>
 static void launch_tree(const TreeArgs& a, hipStream_t st) {
   const TreePlan p = tree_plan(a.rows, a.cache.kvh, a.total, HD, T);
@@ -1207,11 +1218,12 @@ static void launch_tree(const TreeArgs& a, hipStream_t st) {
     }
   } else {
     if constexpr (HD <= 128) {
-      if (p.tiles == 2) RF_KLAUNCH((tree_mfma<T, HD, 2>), grid, dim3(64 * tree_wide(T, HD, 2)), 0, st, a);
+      if (p.tiles == 2) RF_KLAUNCH((tree_mfma<T, HD, 2>), grid, dim3(64 * tree_wide(T, HD, 2)), 0, st, TREE_FIRST, a);
     }
-    if (p.tiles == 1) RF_KLAUNCH((tree_mfma<T, HD, 1>), grid, wg, 0, st, a);
+    if (p.tiles == 1) RF_KLAUNCH((tree_mfma<T, HD, 1>), grid, wg, 0, st, TREE_FIRST, a);
   }
-  if (a.nsplit > 1) RF_KLAUNCH(tree_join<HD>, dim3(a.n * a.qh), dim3(256), 0, st, a);
+  if (a.nsplit > 1)
+    RF_KLAUNCH(tree_join<HD>, dim3(a.n * a.qh), dim3(256), 0, st, a.ws, a.out, a.out_stride, a.n * a.qh, a.qh, a.nsplit);
 }
 
 template <uint32_t T>
