@@ -225,3 +225,40 @@ def test_a_step_captured(ctx, t):
         g.close()
     for c in made:
         c.free()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=lambda t: GGML.NAMES[t])
+@pytest.mark.parametrize("n, hist, kvh, hd", [(6, 700, 2, 128), (40, 64, 1, 64), (9, 50, 1, 160), (64, 4097, 1, 64),
+                                              (1024, 42000, 1, 64)])
+def test_queries_that_are_not_finite(ctx, t, n, hist, kvh, hd):
+    """A NaN or infinity in a query makes its own row's output NaN and reaches no other row."""
+    rng = np.random.default_rng(n)
+    qh = kvh if n > 1000 else 4 * kvh
+    cache, k, v = big_cache(ctx, rng, t, hist + n, kvh, hd)
+    q = rng.standard_normal((n, qh, hd), np.float32)
+    q[1, 0, 5], q[4, qh - 1, hd - 1], q[n - 2, 0, 0] = np.nan, np.inf, -np.inf
+    q[3, 0] = 0
+    out = rf.attention_tree(ctx, ctx.array(q), cache, hist, n, qh).numpy().reshape(n, qh, hd)
+    bad = {(1, 0), (4, qh - 1), (n - 2, 0)}
+    assert all(np.isnan(out[i, h]).all() for i, h in bad)
+    every = [(i, h) for i in range(n) for h in range(qh) if (i, h) not in bad]
+    pairs = every[:60] + every[-60:]
+    check(np.stack([out[i, h] for i, h in pairs]), *some_rows(q, k, v, hist, np.tri(n, dtype=bool), pairs))
+    cache.free()
+
+
+def test_many_steps_on_two_streams_in_order(ctx):
+    """Calls that alternate between two streams, ordered by waiting for each, share the attention workspace."""
+    rng = np.random.default_rng(9)
+    t, kvh, hd, qh, n, hist = GGML.Q8_0, 2, 64, 8, 8, 2500
+    cache, k, v = big_cache(ctx, rng, t, hist + n, kvh, hd)
+    q = [rng.standard_normal((n, qh, hd), np.float32) for _ in range(4)]
+    dev, outs = [ctx.array(x) for x in q], [ctx.empty((n, qh * hd)) for _ in q]
+    for _ in range(3):
+        for i in range(4):
+            rf.attention_tree(ctx, dev[i], cache, hist, n, qh, out=outs[i], stream=ctx.copy_stream if i % 2 else None)
+            ctx.synchronize()
+    pairs = [(i, h) for i in range(n) for h in range(qh)]
+    for x, o in zip(q, outs):
+        check(o.numpy().reshape(-1, hd), *some_rows(x, k, v, hist, np.tri(n, dtype=bool), pairs))
+    cache.free()
