@@ -262,3 +262,36 @@ def test_many_steps_on_two_streams_in_order(ctx):
     for x, o in zip(q, outs):
         check(o.numpy().reshape(-1, hd), *some_rows(x, k, v, hist, np.tri(n, dtype=bool), pairs))
     cache.free()
+
+
+@pytest.mark.parametrize("n, offset", [(8500000, 0), (2100003, 1)], ids=["vector", "any"])
+def test_more_rows_than_one_grid(ctx, n, offset):
+    """Stores and loads of more rows than 65536 workgroups take at once, by both kernels: every row comes back."""
+    w = 32
+    block = np.random.default_rng(n).standard_normal(1000003, np.float32)
+    x = np.resize(block, n * w + offset)
+    d = ctx.array(x)
+    cache = rf.KvCache(ctx, GGML.F32, n, 1, w)
+    rf.kv_store(ctx, cache, d.ptr + 4 * offset, d.ptr + 4 * offset, 0, n)
+    d.upload(np.zeros_like(x))
+    rf.kv_load(ctx, cache, 0, n, d.ptr + 4 * offset, d.ptr + 4 * offset)
+    assert np.array_equal(d.numpy()[offset:], x[offset:])
+    d.free()
+    cache.free()
+
+
+def test_more_tokens_than_one_grid(ctx):
+    """Norm and rotation of 70001 tokens: the last equal a call of their own."""
+    rng = np.random.default_rng(1)
+    n, qh, kvh, hd, m = 70001, 2, 1, 16, 4500
+    q, k = rng.standard_normal((n, qh * hd), np.float32), rng.standard_normal((n, kvh * hd), np.float32)
+    pos = rng.integers(0, 1 << 17, n).astype(np.uint32)
+    got = []
+    for at in (0, n - m):
+        c = n - at
+        qo, ko = ctx.empty((c, qh * hd)), ctx.empty((c, kvh * hd))
+        rf.qk_norm_rope(ctx, ctx.array(q[at:]), ctx.array(k[at:]), None, None, 1e-6, ctx.array(pos[at:]), c, qh, kvh,
+                        hd, 1e4, qo, ko)
+        got.append((qo.numpy(), ko.numpy()))
+    for a, b in zip(*got):
+        assert np.array_equal(a[n - m:], b)
